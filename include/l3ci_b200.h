@@ -398,6 +398,82 @@ L3CI_API size_t l3ci_flash_decode_exchange_bytes(int32_t ranks, int32_t B, int32
 L3CI_API int l3ci_flash_decode_exchange(const l3ci_flash_decode_args* args, void* const* bufs, int32_t rank,
                                         int32_t ranks, uint32_t epoch, int32_t* status);
 
+/* ------------------------------------------------------------------------------------------
+ * Paged caches.  Keys and values of all sequences share cache_k, cache_v [pages, page_size, Hkv, D] (rows [Hkv, D] dense,
+ * pages cache_sp and tokens cache_st elements apart, the same in both); token p of sequence b lies in row p % page_size of
+ * page page_table[b * table_st + p / page_size].  A batch of new tokens is either B sequences of T tokens each, or, with
+ * `starts` (int32 [B + 1], ascending), packed rows: sequence b has rows [starts[b], starts[b + 1]), and rows from
+ * starts[B] on belong to nobody and are left as they were.  Positions, lengths, starts and tables are read on the device alone,
+ * so that a step can be captured in a CUDA graph; an entry of the table that is not in [0, pages) is a page that is not there.
+ * No counterpart in the reference, whose caches are [maxB, maxLen, Hkv, D] (model.py:105-108).
+ * ------------------------------------------------------------------------------------------ */
+
+/* l3ci_rot_embed_kv_cache_at for a paged cache, and, with q_norm / k_norm (bf16 [D] each, both or neither), the RMS norm of every
+ * query and key head in the same pass:  x <- x * rsqrt(mean(x^2) + eps) * weight  over the D entries of a head, before the rotation, in
+ * fp32 with one rounding at the end.  Without norms the results are those of l3ci_rot_embed_kv_cache_at, bit for bit.
+ * Token t of sequence b is at positions[b] + t, its queries go to q_out (rows q_st apart).  A token whose position lies outside the
+ * rotary table (fp32 [freq_rows, D]) or the sequence's pages, or whose page is not there, is skipped: nothing is written for it.
+ * D a multiple of 8, at most 256. */
+typedef struct l3ci_paged_rope_args {
+  const void* qkv;             /* [B, T, (Hq + 2 Hkv) D] by strides qkv_sb, qkv_st; packed rows: qkv_st apart            */
+  const float* freq_table;
+  const void *q_norm, *k_norm;
+  void* q_out;
+  void *cache_k, *cache_v;
+  const int32_t *page_table, *positions, *starts;   /* starts null: B sequences of T tokens                              */
+  int64_t rows;                /* packed rows (starts given)                                                             */
+  int64_t qkv_sb, qkv_st, q_st, freq_rows, pages, cache_sp, cache_st, table_st;
+  int32_t B, T, Hq, Hkv, D, page_size, max_pages;   /* max_pages: entries of a row of the table                          */
+  float eps;
+  l3ci_stream_t stream;
+} l3ci_paged_rope_args;
+L3CI_API int l3ci_rot_embed_paged_kv_cache(const l3ci_paged_rope_args* args);
+
+/* Causal GQA attention of new tokens, one or many per sequence, over a paged cache that holds them already: with n new tokens
+ * of a sequence of seq_lens[b] tokens, token t sees keys j <= seq_lens[b] - n + t.  Lengths are clamped to what the row of the table
+ * can hold; a token that sees no key gets zeros.  Rows of a page behind the sequence's end are not looked at, whatever they hold,
+ * nor does a value that a token must not see (not even one that is no number) reach its result.  Keys and values of a page that is not there count as zeros.
+ * D 64 or 128, Hq / Hkv 1 to 16, page_size a multiple of 16.  scratch: l3ci_paged_attention_scratch_bytes, on 16 bytes, needs no
+ * initialisation; two calls that overlap on the GPU must not share it. */
+typedef struct l3ci_paged_attention_args {
+  const void* q;               /* [B, T, Hq, D] by strides; packed rows [rows, Hq, D] by q_st, q_sh                       */
+  const void *cache_k, *cache_v;
+  void* out;                   /* as q, by strides of its own                                                            */
+  const int32_t *page_table, *seq_lens, *starts;
+  void* scratch;
+  size_t scratch_bytes;
+  int32_t* status;             /* optional device word: L3CI_ERR_DEVICE_WAIT when a bounded wait runs out                */
+  int64_t rows;
+  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, pages, cache_sp, cache_st, table_st;
+  int32_t B, T, Hq, Hkv, D, page_size, max_pages;
+  float scale;                 /* <= 0: 1/sqrt(D)                                                                        */
+  l3ci_stream_t stream;
+} l3ci_paged_attention_args;
+L3CI_API int l3ci_paged_attention(const l3ci_paged_attention_args* args);
+/* Bytes of scratch the call wants on the current device (0: none, or sizes that the call would refuse). */
+L3CI_API size_t l3ci_paged_attention_scratch_bytes(const l3ci_paged_attention_args* args);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[r] = x[r] w^T + scales[i] (x[r] a[i]^T) b[i]^T,   i = index[r];   i outside [0, adapters): the shared product alone.
+ * x bf16 [rows, K] (x_st apart), w bf16 [N, K], a bf16 [adapters, rank, K], b bf16 [adapters, N, rank], all dense, scales fp32
+ * [adapters] (null: 1), index int32 [rows] on the device; out bf16 [rows, N] (out_st apart).  Sums in fp32, one rounding at the end.
+ * K and N multiples of 8, rank a multiple of 8 up to 128.  scratch: l3ci_adapter_linear_scratch_bytes, as above. */
+#define L3CI_ADAPTER_MAX_RANK 128
+typedef struct l3ci_adapter_linear_args {
+  const void *x, *w, *a, *b;
+  const float* scales;
+  const int32_t* index;
+  void* out;
+  void* scratch;
+  size_t scratch_bytes;
+  int32_t* status;
+  int64_t rows, x_st, out_st;
+  int32_t K, N, rank, adapters;
+  l3ci_stream_t stream;
+} l3ci_adapter_linear_args;
+L3CI_API int l3ci_adapter_linear(const l3ci_adapter_linear_args* args);
+L3CI_API size_t l3ci_adapter_linear_scratch_bytes(const l3ci_adapter_linear_args* args);
+
 #ifdef __cplusplus
 }
 #endif

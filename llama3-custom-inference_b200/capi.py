@@ -24,6 +24,8 @@ EXPORTS = (
     "l3ci_flash_decode_kernel_choice",
     "l3ci_lse_merge", "l3ci_lse_exchange_bytes", "l3ci_lse_exchange_merge", "l3ci_prefill_attention",
     "l3ci_flash_decode_exchange_bytes", "l3ci_flash_decode_exchange",
+    "l3ci_rot_embed_paged_kv_cache", "l3ci_paged_attention", "l3ci_paged_attention_scratch_bytes",
+    "l3ci_adapter_linear", "l3ci_adapter_linear_scratch_bytes",
 )
 
 
@@ -64,6 +66,27 @@ class PrefillArgs(C.Structure):
         ("o_sb", C.c_int64), ("o_sh", C.c_int64), ("o_st", C.c_int64),
         ("scale", C.c_float), ("variant", C.c_int32), ("stream", C.c_void_p),
     ]
+
+
+class PagedRopeArgs(C.Structure):
+    """struct l3ci_paged_rope_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("qkv", "freq_table", "q_norm", "k_norm", "q_out", "cache_k", "cache_v", "page_table", "positions", "starts")] + [
+        (n, C.c_int64) for n in ("rows", "qkv_sb", "qkv_st", "q_st", "freq_rows", "pages", "cache_sp", "cache_st", "table_st")] + [
+        (n, C.c_int32) for n in ("B", "T", "Hq", "Hkv", "D", "page_size", "max_pages")] + [("eps", C.c_float), ("stream", C.c_void_p)]
+
+
+class PagedAttentionArgs(C.Structure):
+    """struct l3ci_paged_attention_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "cache_k", "cache_v", "out", "page_table", "seq_lens", "starts", "scratch")] + [
+        ("scratch_bytes", C.c_size_t), ("status", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("rows", "q_sb", "q_st", "q_sh", "o_sb", "o_st", "o_sh", "pages", "cache_sp", "cache_st", "table_st")] + [
+        (n, C.c_int32) for n in ("B", "T", "Hq", "Hkv", "D", "page_size", "max_pages")] + [("scale", C.c_float), ("stream", C.c_void_p)]
+
+
+class AdapterLinearArgs(C.Structure):
+    """struct l3ci_adapter_linear_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "a", "b", "scales", "index", "out", "scratch")] + [("scratch_bytes", C.c_size_t), ("status", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("rows", "x_st", "out_st")] + [(n, C.c_int32) for n in ("K", "N", "rank", "adapters")] + [("stream", C.c_void_p)]
 
 
 class L3ciError(RuntimeError):
@@ -148,6 +171,13 @@ def load() -> C.CDLL:
     lib.l3ci_flash_decode_exchange_bytes.argtypes = [i32, i32, i32, i32]
     lib.l3ci_flash_decode_exchange.restype = C.c_int
     lib.l3ci_flash_decode_exchange.argtypes = [C.POINTER(FlashDecodeArgs), vp, i32, i32, C.c_uint32, vp]
+    for name, args in (("rot_embed_paged_kv_cache", PagedRopeArgs), ("paged_attention", PagedAttentionArgs), ("adapter_linear", AdapterLinearArgs)):
+        getattr(lib, "l3ci_" + name).restype = C.c_int
+        getattr(lib, "l3ci_" + name).argtypes = [C.POINTER(args)]
+    lib.l3ci_paged_attention_scratch_bytes.restype = C.c_size_t
+    lib.l3ci_paged_attention_scratch_bytes.argtypes = [C.POINTER(PagedAttentionArgs)]
+    lib.l3ci_adapter_linear_scratch_bytes.restype = C.c_size_t
+    lib.l3ci_adapter_linear_scratch_bytes.argtypes = [C.POINTER(AdapterLinearArgs)]
     _lib = lib
     return lib
 

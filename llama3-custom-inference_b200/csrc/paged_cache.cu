@@ -1,0 +1,143 @@
+// New tokens into a paged cache (include/l3ci_b200.h, l3ci_rot_embed_paged_kv_cache): one pass over the rows q|k|v of a fused projection
+// norms every query and key head (optional), rotates them, and writes queries to their own rows, keys and values to the tokens' pages.
+//
+// Bound by the bytes of the rows, read once and written once.  One CTA per token: a thread owns one 16-byte vector of a head at a
+// time and sits at the same place of all its heads, so that it loads the rotary table and the norms' weights once; a head's sum of
+// squares is a shuffle over the lanes that hold it.  The row itself does not depend on where the token goes: its loads are asked for
+// before the chain starts -> positions -> page table, which is most of what a decode step's call takes.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "bf16x8.cuh"
+#include "host_common.h"
+#include "ptx_sm100.cuh"
+#include "rotate.cuh"
+#include "warp_reduce.cuh"
+
+namespace l3ci {
+namespace {
+
+constexpr int kBlock = 128;
+constexpr int kBatch = 4;   // 16-byte loads a thread has in flight
+
+// LANES: lanes that hold a head, a power of two of at least D / 8 (those beyond it have nothing).
+template <int LANES, bool NORM>
+__global__ void __launch_bounds__(kBlock)
+rot_embed_paged_kv_cache_kernel(const l3ci_paged_rope_args p) {
+  __shared__ int found;
+  if (threadIdx.x == 0) found = -1;
+  pdl_begin();
+  const long long row = blockIdx.x;
+  int b = p.starts ? 0 : (int)(row / p.T);
+  long long t = p.starts ? 0 : row % p.T;
+  const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(p.qkv) + (p.starts ? row * p.qkv_st : b * p.qkv_sb + t * p.qkv_st);
+  const int vecs = p.D / kVecElems, vec = threadIdx.x % LANES, head0 = threadIdx.x / LANES;
+  constexpr int kHeads = kBlock / LANES;                       // heads the CTA takes at a time
+  const int heads = p.Hq + 2 * p.Hkv;
+  const bool mine = vec < vecs;
+  uint4 v[kBatch];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int h = h0 + u * kHeads;
+      v[u] = mine && h < heads ? ld_stream16(in + h * p.D + vec * kVecElems) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(head0);
+  if (p.starts) {
+    __syncthreads();                                           // (found is set)
+    for (int i = threadIdx.x; i < p.B; i += kBlock)
+      if (__ldg(p.starts + i) <= row && row < __ldg(p.starts + i + 1)) found = i;
+    __syncthreads();
+    b = found;
+    if (b < 0) return;                                         // a row of no sequence
+    t = row - __ldg(p.starts + b);
+  }
+  const long long pos = (long long)__ldg(p.positions + b) + t;
+  if (pos < 0 || pos >= p.freq_rows) return;
+  const long long slot = pos / p.page_size;
+  if (slot >= p.max_pages) return;
+  const int page = __ldg(p.page_table + b * p.table_st + slot);
+  if (page < 0 || page >= p.pages) return;
+  float4 f0 = make_float4(0, 0, 0, 0), f1 = f0;
+  float wq[8] = {}, wk[8] = {};
+  if (mine) {
+    const float* f = p.freq_table + pos * p.D + vec * kVecElems;
+    f0 = __ldg(reinterpret_cast<const float4*>(f));
+    f1 = __ldg(reinterpret_cast<const float4*>(f) + 1);
+    if (NORM) {
+      unpack8(__ldg(static_cast<const uint4*>(p.q_norm) + vec), wq);
+      unpack8(__ldg(static_cast<const uint4*>(p.k_norm) + vec), wk);
+    }
+  }
+  __nv_bfloat16* qo = static_cast<__nv_bfloat16*>(p.q_out) + row * p.q_st + vec * kVecElems;
+  const long long at = page * p.cache_sp + (pos - slot * p.page_size) * p.cache_st + vec * kVecElems;
+  __nv_bfloat16* ko = static_cast<__nv_bfloat16*>(p.cache_k) + at;
+  __nv_bfloat16* vo = static_cast<__nv_bfloat16*>(p.cache_v) + at;
+  // (all lanes of a warp take every round: the shuffles of a norm want them)
+  for (int h0 = head0;; h0 += kHeads * kBatch) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int h = h0 + u * kHeads;
+      uint4 r = v[u];
+      if (NORM) {
+        float a[8], o[8];
+        unpack8(r, a);
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], ss);
+        const float rs = rsqrtf(group_sum<LANES>(ss) / (float)p.D + p.eps);
+        const bool is_q = h < p.Hq;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = a[i] * rs * (is_q ? wq[i] : wk[i]);
+        rotate_pair(a[0], a[1], f0.x, f0.y, o[0], o[1]);
+        rotate_pair(a[2], a[3], f0.z, f0.w, o[2], o[3]);
+        rotate_pair(a[4], a[5], f1.x, f1.y, o[4], o[5]);
+        rotate_pair(a[6], a[7], f1.z, f1.w, o[6], o[7]);
+        if (h < p.Hq + p.Hkv) r = pack8(o);
+      } else if (h < p.Hq + p.Hkv) {
+        r = rotate8(r, f0, f1);
+      }
+      if (!mine || h >= heads) continue;
+      if (h < p.Hq) st_stream16(qo + h * p.D, r);
+      // (the cache rows are read again by the attention of the same step: plain stores)
+      else if (h < p.Hq + p.Hkv) *reinterpret_cast<uint4*>(ko + (h - p.Hq) * p.D) = r;
+      else *reinterpret_cast<uint4*>(vo + (h - p.Hq - p.Hkv) * p.D) = r;
+    }
+    if (h0 - head0 + kHeads * kBatch >= heads) break;
+    load(h0 + kHeads * kBatch);
+  }
+}
+
+}  // namespace
+}  // namespace l3ci
+
+extern "C" int l3ci_rot_embed_paged_kv_cache(const l3ci_paged_rope_args* a) {
+  using namespace l3ci;
+  clear_error();
+  if (!a) return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: null arguments");
+  if (a->B < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->D <= 0 || a->page_size <= 0 || a->max_pages < 0 || a->pages < 0 || a->freq_rows < 0 ||
+      (a->starts ? a->rows < 0 : a->T < 0))
+    return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: B=%d T=%d rows=%lld heads %d, %d of %d, pages of %d", a->B, a->T, (long long)a->rows, a->Hq,
+                a->Hkv, a->D, a->page_size);
+  const long long rows = a->starts ? a->rows : (long long)a->B * a->T;
+  if (rows == 0 || a->B == 0) return L3CI_OK;
+  if (!a->qkv || !a->freq_table || !a->q_out || !a->cache_k || !a->cache_v || !a->page_table || !a->positions || !a->q_norm != !a->k_norm)
+    return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: null pointer");
+  if (a->D % kVecElems || a->D > 256)
+    return fail(L3CI_ERR_UNSUPPORTED, "rot_embed_paged_kv_cache: head size %d is not a multiple of 8 up to 256", a->D);
+  if (!aligned16(a->qkv) || !aligned16(a->freq_table) || !aligned16(a->q_out) || !aligned16(a->cache_k) || !aligned16(a->cache_v) || !aligned16(a->q_norm) ||
+      !aligned16(a->k_norm) || a->qkv_sb % kVecElems || a->qkv_st % kVecElems || a->q_st % kVecElems || a->cache_sp % kVecElems || a->cache_st % kVecElems)
+    return fail(L3CI_ERR_ALIGNMENT, "rot_embed_paged_kv_cache: rows must start on 16 bytes");
+  if (rows > 0x7fffffffLL || ((long long)a->Hq + 2LL * a->Hkv) * a->D > 0x7fffffffLL)
+    return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: tensor too large");
+  if (rows > 1 && a->q_st < (long long)a->Hq * a->D) return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: rows of the queries overlap");
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
+  auto go = [&](auto kernel) -> int {
+    L3CI_LAUNCH("rot_embed_paged_kv_cache_kernel", kernel, dim3((unsigned)rows), dim3(kBlock), 0, stream, *a);
+    return L3CI_OK;
+  };
+  if (a->D <= 64) return a->q_norm ? go(rot_embed_paged_kv_cache_kernel<8, true>) : go(rot_embed_paged_kv_cache_kernel<8, false>);
+  if (a->D <= 128) return a->q_norm ? go(rot_embed_paged_kv_cache_kernel<16, true>) : go(rot_embed_paged_kv_cache_kernel<16, false>);
+  return a->q_norm ? go(rot_embed_paged_kv_cache_kernel<32, true>) : go(rot_embed_paged_kv_cache_kernel<32, false>);
+}

@@ -622,6 +622,156 @@ std::optional<Tensor> linear_rot_embed_kv_cache(Tensor x, Tensor w, Tensor freq,
   return q;
 }
 
+// What the calls on a paged cache share: caches [pages, page_size, n_kv_head, D] of equal layout, a table [B, entries] of page numbers, and
+// new tokens either as [B, T, ...] or, with `starts` (int32 [B + 1]), as packed rows.
+void check_paged(const Tensor& x, const Tensor& cache_k, const Tensor& cache_v, const Tensor& page_table, const Tensor& lengths, const char* lengths_name,
+                 const std::optional<Tensor>& starts) {
+  check_bf16_cuda(cache_k, "cache_k");
+  check_bf16_cuda(cache_v, "cache_v");
+  TORCH_CHECK(cache_k.dim() == 4 && cache_k.sizes() == cache_v.sizes() && cache_k.strides() == cache_v.strides(),
+              "cache_k and cache_v must be [pages, page_size, n_kv_head, D] with equal layout");
+  TORCH_CHECK((cache_k.stride(3) == 1 || cache_k.size(3) == 1) && (cache_k.stride(2) == cache_k.size(3) || cache_k.size(2) == 1), "cache rows must be [n_kv_head, D] contiguous");
+  TORCH_CHECK(page_table.is_cuda() && page_table.scalar_type() == torch::kInt32 && page_table.dim() == 2 && (page_table.stride(1) == 1 || page_table.size(1) <= 1),
+              "page_table must be an int32 CUDA tensor [B, entries] with contiguous rows");
+  const int64_t B = page_table.size(0);
+  TORCH_CHECK(lengths.is_cuda() && lengths.scalar_type() == torch::kInt32 && lengths.dim() == 1 && lengths.size(0) == B && lengths.is_contiguous(), lengths_name,
+              " must be a contiguous int32 CUDA tensor of shape [B]");
+  if (starts) {
+    TORCH_CHECK(starts->is_cuda() && starts->scalar_type() == torch::kInt32 && starts->dim() == 1 && starts->size(0) == B + 1 && starts->is_contiguous(),
+                "starts must be a contiguous int32 CUDA tensor of shape [B + 1]");
+  } else {
+    TORCH_CHECK(x.size(0) == B, "the table must have a row for every sequence");
+  }
+  for (const Tensor* t : {&cache_k, &cache_v, &page_table, &lengths}) TORCH_CHECK(t->get_device() == x.get_device(), "tensors on different devices");
+  TORCH_CHECK(!starts || starts->get_device() == x.get_device(), "tensors on different devices");
+  TORCH_CHECK(B <= INT32_MAX && cache_k.size(1) <= INT32_MAX && cache_k.size(2) <= INT32_MAX && page_table.size(1) <= INT32_MAX, "tensor too large");
+}
+
+// rot_embed_kv_cache for a paged cache: qkv [B, T, (n_head + 2 n_kv_head) D], or packed rows [rows, ...] with `starts`; token t of sequence b is at
+// positions[b] + t of the whole table `freq`.  With q_norm and k_norm (bf16 [D]) every query and key head is normed (RMS, eps) before it is rotated.  Returns the
+// queries [..., n_head, D] (`out`: where they go); a token without a place in the table or the pages is skipped, as rows behind the last sequence are.
+Tensor rot_embed_paged_kv_cache(Tensor qkv, Tensor freq, Tensor cache_k, Tensor cache_v, Tensor page_table, Tensor positions, int64_t n_head, int64_t n_kv_head,
+                                std::optional<Tensor> starts, std::optional<Tensor> q_norm, std::optional<Tensor> k_norm, double eps, std::optional<Tensor> out) {
+  check_bf16_cuda(qkv, "qkv");
+  TORCH_CHECK(qkv.dim() == (starts ? 2 : 3) && (qkv.stride(-1) == 1 || qkv.size(-1) == 1),
+              "qkv must be [B, T, (n_head + 2*n_kv_head) * D], with starts [rows, (n_head + 2*n_kv_head) * D], with a contiguous last dimension");
+  TORCH_CHECK(n_head > 0 && n_kv_head > 0 && n_head <= INT32_MAX && n_kv_head <= INT32_MAX && qkv.size(-1) > 0 && qkv.size(-1) % (n_head + 2 * n_kv_head) == 0,
+              "qkv width does not match the head counts");
+  check_paged(qkv, cache_k, cache_v, page_table, positions, "positions", starts);
+  const int64_t D = qkv.size(-1) / (n_head + 2 * n_kv_head);
+  TORCH_CHECK(cache_k.size(2) == n_kv_head && cache_k.size(3) == D, "the cache's rows must be [n_kv_head, D] of qkv");
+  TORCH_CHECK(freq.is_cuda() && freq.scalar_type() == torch::kFloat32 && freq.dim() == 2 && freq.size(1) == D && freq.is_contiguous() &&
+                  freq.get_device() == qkv.get_device(),
+              "freq must be the whole float32 [rows, D] table, contiguous, on the device of qkv");
+  TORCH_CHECK(q_norm.has_value() == k_norm.has_value(), "q_norm and k_norm go together");
+  if (q_norm) {
+    for (const Tensor* w : {&*q_norm, &*k_norm}) {
+      check_bf16_cuda(*w, "q_norm and k_norm");
+      TORCH_CHECK(w->dim() == 1 && w->size(0) == D && w->is_contiguous() && w->get_device() == qkv.get_device(), "q_norm and k_norm must be contiguous [D] on the device of qkv");
+    }
+  }
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  auto sizes = qkv.sizes().vec();
+  sizes.back() = n_head;
+  sizes.push_back(D);
+  Tensor q = out ? *out : torch::empty(sizes, qkv.options());
+  if (out) {
+    check_bf16_cuda(q, "out");
+    TORCH_CHECK(q.sizes() == torch::IntArrayRef(sizes) && q.is_contiguous() && q.get_device() == qkv.get_device(), "out must be a contiguous [..., n_head, D] on the device of qkv");
+  }
+  l3ci_paged_rope_args a{};
+  a.qkv = qkv.data_ptr(); a.freq_table = freq.data_ptr<float>();
+  a.q_norm = q_norm ? q_norm->data_ptr() : nullptr; a.k_norm = k_norm ? k_norm->data_ptr() : nullptr;
+  a.q_out = q.data_ptr(); a.cache_k = cache_k.data_ptr(); a.cache_v = cache_v.data_ptr();
+  a.page_table = page_table.data_ptr<int32_t>(); a.positions = positions.data_ptr<int32_t>(); a.starts = starts ? starts->data_ptr<int32_t>() : nullptr;
+  a.rows = starts ? qkv.size(0) : 0;
+  a.qkv_sb = starts ? 0 : qkv.stride(0); a.qkv_st = qkv.stride(-2); a.q_st = n_head * D;
+  a.freq_rows = freq.size(0); a.pages = cache_k.size(0); a.cache_sp = cache_k.stride(0); a.cache_st = cache_k.stride(1); a.table_st = page_table.stride(0);
+  a.B = (int32_t)page_table.size(0); a.T = starts ? 0 : (int32_t)qkv.size(1); a.Hq = (int32_t)n_head; a.Hkv = (int32_t)n_kv_head; a.D = (int32_t)D;
+  a.page_size = (int32_t)cache_k.size(1); a.max_pages = (int32_t)page_table.size(1);
+  a.eps = (float)eps;
+  a.stream = current_stream();
+  check_status(l3ci_rot_embed_paged_kv_cache(&a), "rot_embed_paged_kv_cache");
+  return q;
+}
+
+// Attention of new tokens over a paged cache that holds them already: query [B, T, Hq, D], or packed rows [rows, Hq, D] with `starts`; seq_lens
+// counts the new tokens too, and token t of n sees keys j <= seq_lens[b] - n + t.  Returns a tensor like query (`out`: where it goes; rows
+// behind the last sequence keep what they held).
+Tensor paged_attention(Tensor query, Tensor cache_k, Tensor cache_v, Tensor page_table, Tensor seq_lens, std::optional<Tensor> starts, std::optional<Tensor> out,
+                       double scale) {
+  check_bf16_cuda(query, "query");
+  TORCH_CHECK(query.dim() == (starts ? 3 : 4) && (query.stride(-1) == 1 || query.size(-1) == 1), "query must be [B, T, Hq, D], with starts [rows, Hq, D], with a contiguous last dimension");
+  check_paged(query, cache_k, cache_v, page_table, seq_lens, "seq_lens", starts);
+  TORCH_CHECK(cache_k.size(3) == query.size(-1), "head size of query and cache differ");
+  const c10::cuda::CUDAGuard guard(query.device());
+  Tensor y = out ? *out : torch::empty(query.sizes(), query.options());
+  if (out) {
+    check_bf16_cuda(y, "out");
+    TORCH_CHECK(y.sizes() == query.sizes() && y.get_device() == query.get_device() && (y.stride(-1) == 1 || y.size(-1) == 1), "out must be shaped like query, on its device");
+  }
+  l3ci_paged_attention_args a{};
+  a.q = query.data_ptr(); a.cache_k = cache_k.data_ptr(); a.cache_v = cache_v.data_ptr(); a.out = y.data_ptr();
+  a.page_table = page_table.data_ptr<int32_t>(); a.seq_lens = seq_lens.data_ptr<int32_t>(); a.starts = starts ? starts->data_ptr<int32_t>() : nullptr;
+  a.rows = starts ? query.size(0) : 0;
+  a.q_sb = starts ? 0 : query.stride(0); a.q_st = query.stride(-3); a.q_sh = query.stride(-2);
+  a.o_sb = starts ? 0 : y.stride(0); a.o_st = y.stride(-3); a.o_sh = y.stride(-2);
+  a.pages = cache_k.size(0); a.cache_sp = cache_k.stride(0); a.cache_st = cache_k.stride(1); a.table_st = page_table.stride(0);
+  a.B = (int32_t)page_table.size(0); a.T = starts ? 0 : (int32_t)query.size(1); a.Hq = (int32_t)query.size(-2); a.Hkv = (int32_t)cache_k.size(2); a.D = (int32_t)query.size(-1);
+  a.page_size = (int32_t)cache_k.size(1); a.max_pages = (int32_t)page_table.size(1);
+  a.scale = (float)scale;
+  a.stream = current_stream();
+  // (scratch of its own for every call: a captured call's lies in its graph's memory, and no two calls share any)
+  a.scratch_bytes = l3ci_paged_attention_scratch_bytes(&a);
+  Tensor scratch;
+  if (a.scratch_bytes) {
+    scratch = torch::empty({(int64_t)a.scratch_bytes}, query.options().dtype(torch::kUInt8));
+    a.scratch = scratch.data_ptr();
+  }
+  check_status(l3ci_paged_attention(&a), "paged_attention");
+  return y;
+}
+
+// x w^T, and beside it every row's adapter: + scales[i] (x a[i]^T) b[i]^T with i = index[row], none where i is outside [0, adapters).
+// x [..., K], w [N, K], a [adapters, rank, K], b [adapters, N, rank], index int32 over the rows of x.
+Tensor adapter_linear(Tensor x, Tensor w, Tensor a, Tensor b, Tensor index, std::optional<Tensor> scales) {
+  check_bf16_cuda(x, "x");
+  check_bf16_cuda(w, "w");
+  check_bf16_cuda(a, "a");
+  check_bf16_cuda(b, "b");
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "w must be [N, K] with K the last axis of x");
+  TORCH_CHECK(a.dim() == 3 && a.size(2) == x.size(-1), "a must be [adapters, rank, K]");
+  TORCH_CHECK(b.dim() == 3 && b.size(0) == a.size(0) && b.size(1) == w.size(0) && b.size(2) == a.size(1), "b must be [adapters, N, rank]");
+  const int64_t K = x.size(-1), N = w.size(0), rows = K ? x.numel() / K : 0;
+  TORCH_CHECK(index.is_cuda() && index.scalar_type() == torch::kInt32 && index.is_contiguous() && index.numel() == rows, "index must be a contiguous int32 CUDA tensor, one entry per row of x");
+  TORCH_CHECK(!scales || (scales->is_cuda() && scales->scalar_type() == torch::kFloat32 && scales->is_contiguous() && scales->numel() == a.size(0)),
+              "scales must be a contiguous float32 CUDA tensor, one entry per adapter");
+  for (const Tensor* t : {&w, &a, &b, &index}) TORCH_CHECK(t->get_device() == x.get_device(), "tensors on different devices");
+  TORCH_CHECK(!scales || scales->get_device() == x.get_device(), "tensors on different devices");
+  TORCH_CHECK(w.is_contiguous() && a.is_contiguous() && b.is_contiguous(), "w, a and b must be contiguous");
+  TORCH_CHECK(K > 0 && K <= INT32_MAX && N <= INT32_MAX && a.size(0) <= INT32_MAX && a.size(1) <= INT32_MAX, "sizes of x, w and a");
+  const int64_t stride = l3ci_row_stride(x.sizes().data(), x.strides().data(), (int32_t)x.dim());
+  TORCH_CHECK(stride >= 0, "the rows of x must lie at one stride, each contiguous");
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  Tensor out = torch::empty(sizes, x.options());
+  l3ci_adapter_linear_args p{};
+  p.x = x.data_ptr(); p.w = w.data_ptr(); p.a = a.data_ptr(); p.b = b.data_ptr(); p.scales = scales ? scales->data_ptr<float>() : nullptr;
+  p.index = index.data_ptr<int32_t>(); p.out = out.data_ptr();
+  p.rows = rows; p.x_st = stride; p.out_st = N;
+  p.K = (int32_t)K; p.N = (int32_t)N; p.rank = (int32_t)a.size(1); p.adapters = (int32_t)a.size(0);
+  p.stream = current_stream();
+  p.scratch_bytes = l3ci_adapter_linear_scratch_bytes(&p);
+  Tensor scratch;
+  if (p.scratch_bytes) {
+    scratch = torch::empty({(int64_t)p.scratch_bytes}, x.options().dtype(torch::kUInt8));
+    p.scratch = scratch.data_ptr();
+  }
+  check_status(l3ci_adapter_linear(&p), "adapter_linear");
+  return out;
+}
+
 // Status of the few-row products on the current stream of `like`'s device: 0, or 6 once after a device-side wait ran out.
 int64_t linear_status(Tensor like) {
   TORCH_CHECK(like.is_cuda(), "like must be a CUDA tensor");
@@ -677,6 +827,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rot_embed_kv_cache", torch::wrap_pybind_function(rot_embed_kv_cache), "rot_embed_kv_cache",
         py::arg("qkv"), py::arg("freq"), py::arg("cache_k"), py::arg("cache_v"), py::arg("start_pos"),
         py::arg("n_head"), py::arg("n_kv_head"), py::kw_only(), py::arg("positions") = py::none());
+  m.def("rot_embed_paged_kv_cache", torch::wrap_pybind_function(rot_embed_paged_kv_cache), "rot_embed_paged_kv_cache", py::arg("qkv"), py::arg("freq"),
+        py::arg("cache_k"), py::arg("cache_v"), py::arg("page_table"), py::arg("positions"), py::arg("n_head"), py::arg("n_kv_head"), py::kw_only(),
+        py::arg("starts") = py::none(), py::arg("q_norm") = py::none(), py::arg("k_norm") = py::none(), py::arg("eps") = 1e-5, py::arg("out") = py::none());
+  m.def("paged_attention", torch::wrap_pybind_function(paged_attention), "paged_attention", py::arg("query"), py::arg("cache_k"), py::arg("cache_v"),
+        py::arg("page_table"), py::arg("seq_lens"), py::kw_only(), py::arg("starts") = py::none(), py::arg("out") = py::none(), py::arg("scale") = 0.0);
+  m.def("adapter_linear", torch::wrap_pybind_function(adapter_linear), "adapter_linear", py::arg("x"), py::arg("w"), py::arg("a"), py::arg("b"),
+        py::arg("index"), py::kw_only(), py::arg("scales") = py::none());
   m.def("flash_attention_decode_partial", torch::wrap_pybind_function(flash_attention_decode_partial),
         "flash_attention_decode_partial", py::arg("query"), py::arg("keys"), py::arg("values"), py::kw_only(),
         py::arg("seq_lens") = py::none(), py::arg("scale") = 0.0, py::arg("max_ctas") = 0,
