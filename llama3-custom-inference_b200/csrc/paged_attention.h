@@ -1,0 +1,53 @@
+// What the kernels of attention over a paged cache share: the call, the sequences they take, and how work is dealt.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "host_common.h"
+
+namespace l3ci {
+
+// Sequences of one launch (more go in several): their prefix sums lie in shared memory.
+constexpr int kPagedMaxSeqs = 4096;
+
+struct PagedParams {
+  l3ci_paged_attention_args a;
+  int R;               // query heads of a KV head
+  int cap;             // keys that a row of the table can hold
+  int min_rows, max_rows;   // query rows (tokens x R) of the sequences that the launch takes
+  int max_parts;       // CTAs or warps that work is dealt to
+  float scale_log2e;
+  int* pref;           // scratch: columns before each sequence [B + 1]
+  float* records;      // scratch: partial results
+};
+
+struct PagedSeq {
+  int n, len;          // new tokens, keys
+};
+
+#if defined(__CUDACC__)
+// New tokens and keys of sequence b; no tokens where `starts` does not name rows of the call.
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+  PagedSeq s;
+  s.len = min(max(__ldg(p.a.seq_lens + b), 0), p.cap);
+  s.n = p.a.T;
+  if (p.a.starts) {
+    const int r0 = __ldg(p.a.starts + b), r1 = __ldg(p.a.starts + b + 1);
+    s.n = r0 >= 0 && r1 >= r0 && r1 <= p.a.rows ? r1 - r0 : 0;
+  }
+  const long long rows = (long long)s.n * p.R;
+  if (rows < p.min_rows || rows > p.max_rows) s.n = 0;
+  return s;
+}
+// Elements before the first new token of sequence b in a tensor of these strides.
+__device__ __forceinline__ long long paged_row0(const PagedParams& p, int b, long long sb, long long st) {
+  return p.a.starts ? __ldg(p.a.starts + b) * st : b * sb;
+}
+#endif
+
+// paged_attention_tc.cu
+size_t paged_chunks_scratch_bytes(const PagedParams& p);
+int paged_chunks_launch(const PagedParams& p, void* scratch, cudaStream_t stream);
+
+}  // namespace l3ci
