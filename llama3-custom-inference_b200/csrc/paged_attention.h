@@ -9,7 +9,7 @@
 namespace l3ci {
 
 // Sequences of one launch (more go in several): their prefix sums lie in shared memory.
-constexpr int kPagedMaxSeqs = 4096;
+constexpr int kPagedMaxSeqs = 2048;
 
 struct PagedParams {
   l3ci_paged_attention_args a;

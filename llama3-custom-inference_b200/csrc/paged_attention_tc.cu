@@ -1,76 +1,728 @@
-// interim
+// Attention of new tokens over a paged cache (include/l3ci_b200.h, l3ci_paged_attention), sequences of more than a few query rows: chunks of
+// prompts.  Bound by the tensor cores (4 D operations per query row and key) and by the instructions of the softmax between the two products.
+//
+// The same pipeline as prefill_tc_persist_kernel (prefill_attention_tc.cu): tcgen05 products with accumulators in tensor memory, a producer
+// warp, an MMA warp, two softmax groups, an output group.  What differs:
+//   * a tile of 128 query rows is 128 / R tokens by the R query heads of a KV head, so that K and V are read once for all of them, whatever R is
+//     (two tiles, e = 0 and 1, share them: a unit);
+//   * keys come page by page: a tile of 128 keys is filled by copies of as many tokens as lie together in every page (a power of two from 16),
+//     each lane of the producer with its own page;
+//   * tiles of keys of all units are dealt in equal runs to the CTAs, by lengths that the device alone knows; a unit that a run's end cuts goes to
+//     scratch as maximum, sum and fp32 products, and paged_chunk_merge_kernel puts the parts together;
+//   * what lies behind a sequence's end in its last page, and values that some rows of a tile must not see, may be no numbers, and a
+//     weight of 0 does not stop them: two guard warps look through V tiles at the diagonal and the end, under the first product and the softmax
+//     of the same tile, take such values out, and the output group adds them to the rows that see them.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 
 #include "bf16x8.cuh"
+#include "flash_decode_plan.h"
 #include "host_common.h"
 #include "paged_attention.h"
 #include "ptx_sm100.cuh"
+#include "tcgen05.cuh"
+#include "tensor_map.h"
 #include "warp_reduce.cuh"
 
 namespace l3ci {
 namespace {
 
+constexpr int kRows = 128;     // query rows of a tile (M of the products)
+constexpr int kKeys = 128;     // keys of a tile
+constexpr int kStages = 2;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = 32 * (4 + kSoftmaxWarps + 4);
+constexpr int kRegsLow = 56, kRegsHigh = 192, kRegsOut = 72;   // of the producer's, the softmax and the output warpgroups
+static_assert(4 * kRegsLow + kSoftmaxWarps * kRegsHigh + 4 * kRegsOut <= 16 * 128, "register re-deal");
+constexpr uint32_t kTmemCols = 512;                            // S_0, S_1 (128 columns each), O_0, O_1 (D columns each)
+constexpr int kMarks = 4;      // the guards are at most three segments ahead of the output (one-tile segments: two in the ring of V, one on its way out)
+constexpr int kMergeThreads = 256;
+constexpr int kMergeItems = 4;                                 // float4 a thread merges
+
+// The unit that part g of the deal begins in the middle of, written by its CTA for the merge; parts 0: none, or its first cut is another part's.
+struct Cut {
+  int b, h, m, first, last, parts;
+  int pad[2];
+};
+
+struct ChunkParams {
+  PagedParams p;
+  Cut* cuts;
+  int tile_tokens;   // tokens of a tile of query rows: 128 / R
+  int box;           // tokens of a copy
+};
+
+// Floats of a part: o[D / 4][256 rows][4], m[256], l[256].
 template <int D>
-__global__ void __launch_bounds__(128) paged_attention_row_kernel(const PagedParams pp) {
-  pdl_begin();
-  const l3ci_paged_attention_args& p = pp.a;
-  const float scale_log2e = pp.scale_log2e;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long long row = item / p.Hq;
-  const int hq = (int)(item % p.Hq), h = hq / (p.Hq / p.Hkv);
-  if (row >= p.rows) return;
-  int b = 0, n = p.T;
-  long long t = 0;
-  if (p.starts) {
-    int hit = -1;
-    for (int i = lane; i < p.B; i += 32)
-      if (p.starts[i] <= row && row < p.starts[i + 1]) hit = i;
-    hit = __reduce_max_sync(kFullMask, hit);
-    if (hit < 0) return;
-    b = hit;
-    t = row - p.starts[b];
-    n = p.starts[b + 1] - p.starts[b];
-  } else {
-    b = (int)(row / p.T);
-    t = row % p.T;
-  }
-  if ((long long)n * pp.R < pp.min_rows || n < 0) return;
-  const long long cap = (long long)p.max_pages * p.page_size;
-  const long long len = min(max((long long)p.seq_lens[b], 0LL), cap);
-  const long long seen = len - n + t + 1;
-  constexpr int E = D / 32;
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + (p.starts ? row * p.q_st : b * p.q_sb + t * p.q_st) + hq * p.q_sh + lane * E;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + (p.starts ? row * p.o_st : b * p.o_sb + t * p.o_st) + hq * p.o_sh + lane * E;
-  float x[E], o[E] = {};
-  for (int i = 0; i < E; ++i) x[i] = __bfloat162float(q[i]);
-  float m = -INFINITY, l = 0.f;
-  for (long long j = 0; j < seen; ++j) {
-    const int page = p.page_table[b * p.table_st + j / p.page_size];
-    const bool there = page >= 0 && page < p.pages;
-    const long long at = page * p.cache_sp + j % p.page_size * p.cache_st + h * D + lane * E;
-    float s = 0.f;
-    for (int i = 0; i < E; ++i) s += x[i] * (there ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.cache_k)[at + i]) : 0.f);
-    s = group_sum<32>(s) * scale_log2e;
-    const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn, a = exp2f(m - mu), e = exp2f(s - mu);
-    l = l * a + e;
-    for (int i = 0; i < E; ++i) o[i] = o[i] * a + e * (there ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.cache_v)[at + i]) : 0.f);
-    m = mn;
-  }
-  for (int i = 0; i < E; ++i) out[i] = __float2bfloat16_rn(seen > 0 ? o[i] / l : 0.f);
+__host__ __device__ constexpr long long part_floats() { return 2 * kRows * (D + 2); }
+template <int D>
+__device__ __forceinline__ float* part_of(const PagedParams& p, int part, bool begins) {
+  return p.records + (2 * part + (begins ? 1 : 0)) * part_floats<D>();
 }
 
+// Keys that the tokens of block m (2 * tile_tokens tokens) of a sequence see, in tiles; at least one.
+__device__ __forceinline__ int unit_tiles(const PagedSeq& s, int m, int block) {
+  const int seen = s.len - s.n + min(s.n, (m + 1) * block);
+  return seen <= 0 ? 1 : (seen + kKeys - 1) / kKeys;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                   const __grid_constant__ ChunkParams cp) {
+  constexpr int kHalves = D / 64;
+  constexpr int kBoxBytes = 128 * 128;             // 128 rows of 128 bytes
+  constexpr int kTileBytes = kHalves * kBoxBytes;  // a Q, K or V tile
+  constexpr int kSPitch = 64 + 16;                 // staging row: 32 output columns + padding
+  const PagedParams& p = cp.p;
+  const l3ci_paged_attention_args& a = p.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_smem = smem_u32(smem);
+  const uint32_t k_smem = q_smem + 2 * kTileBytes;             // [kStages]
+  const uint32_t v_smem = k_smem + kStages * kTileBytes;       // [kStages]
+  uint8_t* stage_all = smem + (2 + 2 * kStages) * kTileBytes;  // [2 tiles][128 rows][kSPitch]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_all + 2 * kRows * kSPitch);
+  // as in prefill_tc_persist_kernel; V_GO: the guard warps may go through a tile of V, which has landed; V_OK: they have
+  enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_GO = 14, V_OK = 15, P_FULL = 16, L_FULL = 18, O_READ = 20,
+         N_BARS = 22 };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
+  int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kMarks]: values taken out of tiles of a segment
+  int* sums = odd + kMarks;                                            // [16 warps]
+  float* stat = reinterpret_cast<float*>(sums + 16);               // [2 tiles][128 rows][l, m_ref]
+  int* pref = reinterpret_cast<int*>(stat + 4 * kRows);            // [B + 1]
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_FULL ? kSoftmaxWarps / 2 : i == V_OK ? 2 : 1);
+    for (int i = 0; i < kMarks; ++i) odd[i] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  // ---- columns (a unit's tile of keys each) before every sequence ----
+  const int block = 2 * cp.tile_tokens;
+  auto columns_of_head = [&](const PagedSeq& s) {
+    int sum = 0;
+    for (int m = 0; m * block < s.n; ++m) sum += unit_tiles(s, m, block);
+    return sum;
+  };
+  {
+    const int each = (a.B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * each, a.B), b1 = min(b0 + each, a.B);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int c = a.Hkv * columns_of_head(paged_seq(p, b));
+      pref[b + 1] = c;
+      mine += c;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(kFullMask, upto, d);
+      if (lane >= d) upto += other;
+    }
+    if (lane == 31) sums[warp] = upto;
+    if (threadIdx.x == 0) pref[0] = 0;
+    __syncthreads();
+    int before = upto - mine;
+    for (int w = 0; w < warp; ++w) before += sums[w];
+    for (int b = b0; b < b1; ++b) pref[b + 1] = before += pref[b + 1];
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t t_s[2] = {tmem, tmem + 128u};
+  const uint32_t t_o[2] = {tmem + 256u, tmem + 256u + (uint32_t)D};
+  const int total = pref[a.B], parts = min(total, p.max_parts), part = blockIdx.x;
+  const int begin = part < parts ? fd_range_begin(part, total, parts) : 0, end = part < parts ? fd_range_begin(part + 1, total, parts) : 0;
+
+  // ---- a CTA's run is a list of segments: tiles [j0, j1) of a unit ----
+  struct Unit { int b, h, m, n, len, first, tiles; };   // first: its first column
+  auto unit_at = [&](int col) {                         // the unit that holds a column
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pref[mid] <= col) lo = mid; else hi = mid;
+    }
+    Unit u;
+    u.b = lo;
+    const PagedSeq s = paged_seq(p, lo);
+    u.n = s.n;
+    u.len = s.len;
+    const int per_head = (pref[lo + 1] - pref[lo]) / a.Hkv, local = col - pref[lo];
+    u.h = local / per_head;
+    int before = u.h * per_head;
+    for (u.m = 0;; ++u.m) {
+      u.tiles = unit_tiles(s, u.m, block);
+      if (before + u.tiles > local) break;
+      before += u.tiles;
+    }
+    u.first = pref[lo] + before;
+    return u;
+  };
+  auto next_unit = [&](Unit& u) {
+    u.first += u.tiles;
+    if (++u.m * block >= u.n) {
+      u.m = 0;
+      if (++u.h == a.Hkv) {
+        u.h = 0;
+        do ++u.b; while (u.b < a.B && pref[u.b + 1] == pref[u.b]);
+        if (u.b >= a.B) return;
+        const PagedSeq s = paged_seq(p, u.b);
+        u.n = s.n;
+        u.len = s.len;
+      }
+    }
+    u.tiles = unit_tiles(PagedSeq{u.n, u.len}, u.m, block);
+  };
+  auto tiles_from = [&](const Unit& u, int col) { return col - u.first; };
+  auto tiles_to = [&](const Unit& u) { return min(u.tiles, end - u.first); };
+  auto both = [&](const Unit& u) { return u.m * block + cp.tile_tokens < u.n; };      // the second tile of rows has tokens
+  auto first_limit = [&](const Unit& u, int e) { return u.len - u.n + u.m * block + e * cp.tile_tokens; };   // last key of the tile's first token
+  auto cut_tile = [&](int j, int limit) { return j * kKeys + kKeys - 1 > limit; };    // some row does not see all keys
+  bool ok = true;
+  int fill = 0;        // tiles of keys so far: stage and phase of the rings follow
+  int segments = 0;
+
+  if (warp == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    // ---- producer: lane 0 the query rows, every lane the tokens of its own copies ----
+    const uint64_t policy = l2_evict_first_policy();
+    const int copies = kKeys / cp.box;                      // per half of a tile
+    Unit u = begin < end ? unit_at(begin) : Unit{};
+    for (int col = begin; col < end && ok; ++segments) {
+      if (segments > 0 && !mbar_wait_bounded(bar(Q_EMPTY), (segments - 1) & 1)) { ok = false; break; }
+      const int t0 = u.m * block;
+      if (lane == 0) {
+        const int tiles = both(u) ? 2 : 1, rows = cp.tile_tokens * p.R;
+        const int row = a.starts ? __ldg(a.starts + u.b) + t0 : t0;
+        mbar_expect_tx(bar(Q_FULL), tiles * kHalves * rows * 128);
+        for (int e = 0; e < tiles; ++e)
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_4d(q_smem + e * kTileBytes + h * kBoxBytes, &qmap, bar(Q_FULL), h * 64, u.h * p.R, row + e * cp.tile_tokens, a.starts ? 0 : u.b, policy);
+      }
+      auto page_of = [&](int j) {                          // of this lane's tokens of tile j; one past the last: nothing is there
+        const int token = j * kKeys + lane * cp.box;
+        const int page = lane < copies && token < u.len ? __ldg(a.page_table + u.b * a.table_st + token / a.page_size) : -1;
+        return page >= 0 && page < a.pages ? page : (int)a.pages;
+      };
+      const int j1 = tiles_to(u);
+      int j = tiles_from(u, col), page = page_of(j);
+      for (; j < j1 && ok; ++j, ++fill) {
+        const int s = fill % kStages, off = (j * kKeys + lane * cp.box) % a.page_size;
+        const int ahead = page_of(j + 1);
+        const uint32_t par = ((fill / kStages) - 1) & 1;
+        if (fill >= kStages && !mbar_wait_bounded(bar(K_EMPTY + s), par)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(bar(K_FULL + s), kTileBytes);
+        __syncwarp();
+        if (lane < copies)
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_4d(k_smem + s * kTileBytes + h * kBoxBytes + lane * cp.box * 128, &kmap, bar(K_FULL + s), h * 64, off, u.h, page, policy);
+        if (fill >= kStages && !mbar_wait_bounded(bar(V_EMPTY + s), par)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(bar(V_FULL + s), kTileBytes);
+        __syncwarp();
+        if (lane < copies)
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_4d(v_smem + s * kTileBytes + h * kBoxBytes + lane * cp.box * 128, &vmap, bar(V_FULL + s), h * 64, off, u.h, page, policy);
+        page = ahead;
+      }
+      col = u.first + j1;
+      if (col < end) next_unit(u);
+    }
+  } else if (warp == 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    // ---- MMA issue: all lanes run the code, one elected lane predicates the instructions ----
+    constexpr uint32_t idesc_qk = instr_desc(kRows, kKeys, false);
+    constexpr uint32_t idesc_pv = instr_desc(kRows, D, true);
+    const uint32_t elected = lane == 0 ? 1u : 0u;
+    const uint64_t q_desc = smem_desc(q_smem, 16, 1024);
+    const uint64_t k_desc = smem_desc(k_smem, 16, 1024);
+    const uint64_t v_desc = smem_desc(v_smem, kBoxBytes, 1024);
+    // S_{e,g} = Q_e K^T (g: tile number over all segments) into tile e's score accumulator
+    auto issue_s = [&](int e, int g, bool last_of_tile, bool last_of_segment) {
+      const int s = g % kStages;
+      const uint64_t qd = q_desc + (uint64_t)((e * kTileBytes) >> 4);
+      const uint64_t kd = k_desc + (uint64_t)((s * kTileBytes) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint64_t step = (uint64_t)(((ks >> 2) * kBoxBytes + (ks & 3) * 32) / 16);
+        mma_ss(t_s[e], qd + step, kd + step, idesc_qk, ks > 0, elected);
+      }
+      tc_commit(bar(S_FULL + e), elected);
+      if (last_of_tile) {
+        tc_commit(bar(K_EMPTY + s), elected);
+        if (last_of_segment) tc_commit(bar(Q_EMPTY), elected);
+      }
+    };
+    int done[2] = {0, 0}, seg_of[2] = {0, 0};   // tiles and segments of each tile of rows
+    int guarded = 0;                          // tiles that the guards have been through
+    Unit u = begin < end ? unit_at(begin) : Unit{};
+    for (int col = begin; col < end && ok; ++segments) {
+      const int j0 = tiles_from(u, col), j1 = tiles_to(u), ne = both(u) ? 2 : 1, limit = first_limit(u, 0);
+      if (!mbar_wait_bounded(bar(Q_FULL), segments & 1)) { ok = false; break; }
+      if (!mbar_wait_bounded(bar(K_FULL + fill % kStages), (fill / kStages) & 1)) { ok = false; break; }
+      tc_fence_after();
+      for (int e = 0; e < ne; ++e) issue_s(e, fill, e == ne - 1, j0 + 1 == j1);
+      for (int j = j0; j < j1 && ok; ++j, ++fill) {
+        const int s = fill % kStages;
+        if (!mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
+        bool guard = false;
+        if (cut_tile(j, limit)) {
+          if (lane == 0) mbar_arrive(bar(V_GO));
+          guard = true;
+        }
+        for (int e = 0; e < ne; ++e) {
+          // O_e += P_e V once P_e is in tensor memory, on a segment's first tile once the last segment's O_e has been read; then at
+          // once the next scores, which go where P_e lay
+          if (!mbar_wait_bounded(bar(P_FULL + e), done[e] & 1)) { ok = false; break; }
+          if (j == j0 && seg_of[e] > 0 && !mbar_wait_bounded(bar(O_READ + e), (seg_of[e] - 1) & 1)) { ok = false; break; }
+          if (guard) {
+            if (!mbar_wait_bounded(bar(V_OK), guarded & 1)) { ok = false; break; }
+            ++guarded;
+            guard = false;
+          }
+          tc_fence_after();
+          const uint64_t vd = v_desc + (uint64_t)((s * kTileBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_ts(t_o[e], t_s[e] + kk * 8, vd + (uint64_t)(kk * 128), idesc_pv, (j > j0 || kk > 0) ? 1u : 0u, elected);
+          tc_commit(bar(O_FULL + e), elected);
+          if (e == ne - 1) tc_commit(bar(V_EMPTY + s), elected);
+          ++done[e];
+          if (j + 1 < j1) {
+            if (e == 0) {
+              if (!mbar_wait_bounded(bar(K_FULL + (fill + 1) % kStages), ((fill + 1) / kStages) & 1)) { ok = false; break; }
+              tc_fence_after();
+            }
+            issue_s(e, fill + 1, e == ne - 1, j + 2 == j1);
+          }
+        }
+      }
+      for (int e = 0; e < ne; ++e) ++seg_of[e];
+      col = u.first + j1;
+      if (col < end) next_unit(u);
+    }
+  } else if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    // ---- guards: two keys' values a thread, tiles at the diagonal and the end only ----
+    int guarded = 0;
+    Unit u = begin < end ? unit_at(begin) : Unit{};
+    for (int col = begin; col < end && ok; ++segments) {
+      const int j1 = tiles_to(u), limit = first_limit(u, 0);
+      for (int j = tiles_from(u, col); j < j1 && ok; ++j, ++fill) {
+        if (!cut_tile(j, limit)) continue;
+        // (not by V_FULL alone: two tiles further on its phase would look the same as two tiles before)
+        const int s = fill % kStages;
+        if (!mbar_wait_bounded(bar(V_GO), guarded++ & 1) || !mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
+        bool any = false;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int r = ((warp - 2) * 2 + i) * 32 + lane;
+          const bool behind = j * kKeys + r >= u.len;
+#pragma unroll 1
+          for (int c = 0; c < kHalves * 8; ++c) {
+            const uint32_t at = v_smem + s * kTileBytes + (c >> 3) * kBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+            bool write = behind;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if (behind) w[x] = 0;
+              if ((w[x] & 0x7f80u) == 0x7f80u) { w[x] &= 0xffff0000u; write = any = true; }
+              if ((w[x] & 0x7f800000u) == 0x7f800000u) { w[x] &= 0xffffu; write = any = true; }
+            }
+            if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          }
+        }
+        if (any) odd[segments % kMarks] = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(V_OK));
+      }
+      col = u.first + j1;
+      if (col < end) next_unit(u);
+    }
+  } else if (warp < 4 + kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    // ---- softmax: group e = tile e of the unit's rows, a thread a row ----
+    const int q4 = warp & 3, e = (warp - 4) >> 2, r = q4 * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
+    const uint32_t ts = t_s[e] + lane_addr, to = t_o[e] + lane_addr;
+    constexpr float kLazy = 8.f;                   // log2 of how far the running maximum may outgrow m_ref
+    const int token = r / p.R;                     // of the tile
+    int g = 0, mine = 0;                           // tiles and segments of this group so far
+    Unit u = begin < end ? unit_at(begin) : Unit{};
+    for (int col = begin; col < end && ok; ++segments) {
+      const int j0 = tiles_from(u, col), j1 = tiles_to(u);
+      if (e == 0 || both(u)) {
+        const int limit0 = first_limit(u, e), limit = token < cp.tile_tokens ? limit0 + token : -1;   // last key this row may see
+        float m_ref = -INFINITY, l_run = 0.f;
+        for (int j = j0; j < j1 && ok; ++j, ++g) {
+          if (!mbar_wait_bounded(bar(S_FULL + e), g & 1)) { ok = false; break; }
+          tc_fence_after();
+          uint32_t x[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, x[c]);
+          tc_wait_ld();
+          if (cut_tile(j, limit0)) {
+            const int left = min(limit, u.len - 1) - j * kKeys;    // last key of the tile that this row sees
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i > left) x[c][i] = 0xff800000u;      // -inf
+          }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              mx4[(i >> 1) & 3] = fmax3(mx4[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e;
+          // the reference maximum moves (and this warp's rows of O_e are rescaled) only when some row needs it
+          if (__any_sync(kFullMask, mx > m_ref + kLazy)) {
+            const float m_new = fmaxf(m_ref, mx);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
+            if (j > j0) {
+              if (!mbar_wait_bounded(bar(O_FULL + e), (g - 1) & 1)) { ok = false; break; }
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t y[32];
+                tmem_ld32(to + c * 32, y);
+                tc_wait_ld();
+                uint32_t lo[16], hi[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  lo[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+                  hi[i] = __float_as_uint(__uint_as_float(y[16 + i]) * alpha);
+                }
+                tmem_st16(to + c * 32, lo);
+                tmem_st16(to + c * 32 + 16, hi);
+              }
+              l_run *= alpha;
+            }
+            m_ref = m_new;
+          }
+          const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+          const unsigned long long scale2 = f2_packf(p.scale_log2e, p.scale_log2e), nmu2 = f2_packf(-mu, -mu);
+          unsigned long long ps2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+            unsigned long long t2[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t2[i] = f2_fma(f2_pack(x[c][2 * i], x[c][2 * i + 1]), scale2, nmu2);
+            float pe[32];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1;
+              f2_unpack(t2[i], x0, x1);
+              pe[2 * i] = fast_exp2(x0);
+              pe[2 * i + 1] = fast_exp2(x1);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              ps2[i & 3] = f2_add(ps2[i & 3], f2_packf(pe[2 * i], pe[2 * i + 1]));
+              pk[i] = pack_bf16x2(pe[2 * i], pe[2 * i + 1]);
+            }
+            tmem_st16(ts + c * 16, pk);                // P: 64 packed columns over the first 64 of S
+          }
+          {
+            float a0, a1, b0, b1;
+            f2_unpack(f2_add(ps2[0], ps2[1]), a0, a1);
+            f2_unpack(f2_add(ps2[2], ps2[3]), b0, b1);
+            l_run += (a0 + a1) + (b0 + b1);
+          }
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(P_FULL + e));
+        }
+        if (!ok) break;
+        // the row's sums go to the output group, which has read the last segment's before it arrived on O_READ
+        if (mine > 0 && !mbar_wait_bounded(bar(O_READ + e), (mine - 1) & 1)) { ok = false; break; }
+        *reinterpret_cast<float2*>(stat + (e * kRows + r) * 2) = make_float2(l_run, m_ref);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L_FULL + e));
+        ++mine;
+      }
+      col = u.first + j1;
+      if (col < end) next_unit(u);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOut));
+    // ---- output: a thread a row of one tile after the other ----
+    const int q4 = warp & 3, r = q4 * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
+    int g[2] = {0, 0}, mine[2] = {0, 0};
+    Unit u = begin < end ? unit_at(begin) : Unit{};
+    if (r == 0) {      // what the merge has to know of the unit that this run begins in the middle of
+      Cut cut = {};
+      if (begin < end && u.first < begin) {
+        cut.first = fd_cta_of(u.first, total, parts);
+        if (cut.first == part - 1) {
+          cut.b = u.b;
+          cut.h = u.h;
+          cut.m = u.m;
+          cut.last = fd_cta_of(u.first + u.tiles - 1, total, parts);
+          cut.parts = cut.last - cut.first + 1;
+        }
+      }
+      cp.cuts[part] = cut;
+    }
+    for (int col = begin; col < end && ok; ++segments) {
+      const int j0 = tiles_from(u, col), j1 = tiles_to(u), ne = both(u) ? 2 : 1;
+      const bool whole = j0 == 0 && j1 == u.tiles;
+      const long long row0 = paged_row0(p, u.b, a.o_sb, a.o_st);
+      for (int e = 0; e < ne && ok; ++e) {
+        if (!mbar_wait_bounded(bar(L_FULL + e), mine[e] & 1)) { ok = false; break; }
+        const float2 lm = *reinterpret_cast<const float2*>(stat + (e * kRows + r) * 2);
+        g[e] += j1 - j0;
+        if (!mbar_wait_bounded(bar(O_FULL + e), (g[e] - 1) & 1)) { ok = false; break; }   // the segment's last product
+        tc_fence_after();
+        const int t0 = u.m * block + e * cp.tile_tokens, tokens = min(cp.tile_tokens, u.n - t0);   // tokens of the tile
+        const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kMarks) != 0;
+        uint8_t* stage = stage_all + e * (kRows * kSPitch);
+        const float inv = lm.x == 0.f ? 0.f : 1.f / lm.x;
+        float* rec = part_of<D>(p, part, j0 == 0);
+        const uint32_t to = t_o[e] + lane_addr;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t y[32];
+          tmem_ld32(to + c * 32, y);
+          tc_wait_ld();
+          if (taken) {
+            // values that the guards took out, for the rows that see them: from the cache, key by key (a call with such values is lost anyway)
+            const int limit = min(first_limit(u, e) + r / p.R, u.len - 1), from = max(j0 * kKeys, (first_limit(u, 0) + 1) / kKeys * kKeys);
+            const int upto = min(limit, j1 * kKeys - 1);
+            if (r < tokens * p.R)
+#pragma unroll 1
+              for (int key = max(from, 0); key <= upto; ++key) {
+                const int page = __ldg(a.page_table + u.b * a.table_st + key / a.page_size);
+                if (page < 0 || page >= a.pages) continue;
+                const uint16_t* v = static_cast<const uint16_t*>(a.cache_v) + page * a.cache_sp + key % a.page_size * a.cache_st + u.h * D + c * 32;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  uint16_t w;
+                  asm volatile("ld.global.u16 %0, [%1];" : "=h"(w) : "l"(v + i));    // (one at a time: registers are few here)
+                  if ((w & 0x7f80) == 0x7f80) y[i] = __float_as_uint(__uint_as_float(y[i]) + __uint_as_float((uint32_t)w << 16));
+                }
+              }
+          }
+          if (whole) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) w[i >> 1] = pack_bf16x2(__uint_as_float(y[i]) * inv, __uint_as_float(y[i + 1]) * inv);
+            uint4* dst = reinterpret_cast<uint4*>(stage + r * kSPitch);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+            asm volatile("bar.sync 2, 128;" ::: "memory");   // the output warpgroup
+#pragma unroll
+            for (int id = r; id < kRows * 4; id += 128) {
+              const int row = id >> 2, ch = id & 3, t = row / p.R;
+              if (t < tokens)
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row0 + (t0 + t) * a.o_st + (long long)(u.h * p.R + row - t * p.R) * a.o_sh + c * 32 + ch * 8) =
+                    *reinterpret_cast<const uint4*>(stage + row * kSPitch + ch * 16);
+            }
+            asm volatile("bar.sync 2, 128;" ::: "memory");   // the rows may be written again
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<uint4*>(rec + ((long long)(c * 8 + q) * (2 * kRows) + e * kRows + r) * 4) = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+          }
+        }
+        if (!whole) {
+          rec[2 * kRows * D + e * kRows + r] = lm.y;
+          rec[2 * kRows * (D + 1) + e * kRows + r] = lm.x;
+        }
+        if (e == ne - 1) {
+          asm volatile("bar.sync 2, 128;" ::: "memory");     // (all have read the mark)
+          if (r == 0) odd[segments % kMarks] = 0;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(O_READ + e));
+        ++mine[e];
+      }
+      col = u.first + j1;
+      if (col < end) next_unit(u);
+    }
+  }
+  if (!ok && lane == 0 && a.status) atomicExch(a.status, (int)L3CI_ERR_DEVICE_WAIT);
+  __syncwarp();
+  tc_fence_before();
+  // a wait ran out: the copies still under way land before the shared memory is given back (or their own waits run out too)
+  if (__syncthreads_or(!ok) && threadIdx.x == 0) {
+    if (segments > 0 || fill > 0) (void)mbar_wait_bounded_one(bar(Q_FULL), segments & 1);
+    for (int f = max(fill - kStages, 0); f <= fill; ++f) {
+      (void)mbar_wait_bounded_one(bar(K_FULL + f % kStages), (f / kStages) & 1);
+      (void)mbar_wait_bounded_one(bar(V_FULL + f % kStages), (f / kStages) & 1);
+    }
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Puts the parts of a cut unit together: blockIdx.x the part that it is cut at first, blockIdx.y a share of its rows and columns.
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads) paged_chunk_merge_kernel(const ChunkParams cp) {
+  const PagedParams& p = cp.p;
+  const l3ci_paged_attention_args& a = p.a;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int4 c0 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + blockIdx.x + 1)), c1 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + blockIdx.x + 1) + 1);
+  const int b = c0.x, h = c0.y, m = c0.z, first = c0.w, parts = c1.y;
+  if (parts < 2) return;
+  const PagedSeq s = paged_seq(p, b);
+  const int t_unit = m * 2 * cp.tile_tokens;
+  const long long row0 = paged_row0(p, b, a.o_sb, a.o_st);
+  // neighbouring lanes: 8 rows of 4 vectors each (runs of 128 bytes of a part, of 32 bytes of the result)
+  constexpr int kPerRow = D / 4;
+#pragma unroll 1
+  for (int i = 0; i < kMergeItems; ++i) {
+    const int item = (blockIdx.y * kMergeItems + i) * kMergeThreads + threadIdx.x;
+    const int in8 = item & 31, rest = item >> 5;
+    const int vec = (rest % (kPerRow / 4)) * 4 + (in8 >> 3), row = rest / (kPerRow / 4) * 8 + (in8 & 7);   // row: 0 .. 255
+    const int e = row / kRows, t = (row % kRows) / p.R, token = t_unit + e * cp.tile_tokens + t;
+    if (t >= cp.tile_tokens || token >= s.n) continue;
+    float mx = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAtOnce = 4;
+    for (int p0 = 0; p0 < parts; p0 += kAtOnce) {
+      float mv[kAtOnce], lv[kAtOnce];
+      float4 ov[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        mv[k] = -INFINITY;
+        lv[k] = 0.f;
+        ov[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p0 + k < parts) {
+          const float* rec = part_of<D>(p, first + p0 + k, p0 + k == 0);
+          ov[k] = __ldcg(reinterpret_cast<const float4*>(rec) + vec * (2 * kRows) + row);
+          mv[k] = __ldcg(rec + 2 * kRows * D + row);
+          lv[k] = __ldcg(rec + 2 * kRows * (D + 1) + row);
+        }
+      }
+      float mn = mx;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, mv[k]);
+      const float mu = mn == -INFINITY ? 0.f : mn, w0 = fast_exp2(mx - mu);
+      l *= w0;
+      acc.x *= w0; acc.y *= w0; acc.z *= w0; acc.w *= w0;
+      mx = mn;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        if (p0 + k >= parts) break;
+        const float w = fast_exp2(mv[k] - mu);
+        l = fmaf(lv[k], w, l);
+        acc.x = fmaf(ov[k].x, w, acc.x);
+        acc.y = fmaf(ov[k].y, w, acc.y);
+        acc.z = fmaf(ov[k].z, w, acc.z);
+        acc.w = fmaf(ov[k].w, w, acc.w);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 + token * a.o_st + (long long)(h * p.R + row % kRows - t * p.R) * a.o_sh;
+    *reinterpret_cast<uint2*>(out + vec * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  }
+}
+
+// ---- host ----
+size_t chunk_smem(int D, int B) {
+  const size_t tile = (size_t)(D / 64) * 128 * 128;
+  return 1024 + 6 * tile + 2 * kRows * 80 + 23 * 8 + (kMarks + 16) * 4 + 4 * kRows * 4 + (size_t)(B + 1) * 4;
+}
+
+int chunk_parts(const PagedParams& p) {
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  // (columns at most: every token's own unit of all the keys that the table can hold)
+  const long long rows = p.a.starts ? p.a.rows : (long long)p.a.B * p.a.T, block = 2 * (kRows / p.R);
+  const long long columns = (rows / block + p.a.B) * p.a.Hkv * (((long long)p.cap + kKeys - 1) / kKeys + 1);
+  return (int)(columns < sms ? columns : sms);
+}
+
+int chunk_maps(const ChunkParams& cp, CUtensorMap* qmap, CUtensorMap* kmap, CUtensorMap* vmap) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(L3CI_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const l3ci_paged_attention_args& a = cp.p.a;
+  const cuuint64_t row = (cuuint64_t)a.D * 2;
+  const cuuint32_t one[4] = {1u, 1u, 1u, 1u};
+  {
+    const long long T = a.starts ? a.rows : a.T, B = a.starts ? 1 : a.B;
+    // (a dimension of extent 1 may carry any stride in the caller's view; a valid one then)
+    const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.Hq, (cuuint64_t)T, (cuuint64_t)B};
+    const cuuint64_t strides[3] = {a.Hq > 1 ? (cuuint64_t)a.q_sh * 2 : row, T > 1 ? (cuuint64_t)a.q_st * 2 : row, B > 1 ? (cuuint64_t)a.q_sb * 2 : row};
+    const cuuint32_t box[4] = {64u, (cuuint32_t)cp.p.R, (cuuint32_t)cp.tile_tokens, 1u};
+    const CUresult r = enc(qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(L3CI_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+  }
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_size, (cuuint64_t)a.Hkv, (cuuint64_t)a.pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.cache_st * 2, row, a.pages > 1 ? (cuuint64_t)a.cache_sp * 2 : row};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)cp.box, 1u, 1u};
+  for (int i = 0; i < 2; ++i) {
+    const CUresult r = enc(i ? vmap : kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(i ? a.cache_v : a.cache_k), dims, strides, box, one,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           a.D == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(L3CI_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+  }
+  return L3CI_OK;
+}
+
+template <int D>
+int chunk_launch(const ChunkParams& cp, cudaStream_t stream) {
+  CUtensorMap qmap, kmap, vmap;
+  if (int st = chunk_maps(cp, &qmap, &kmap, &vmap)) return st;
+  static bool configured[64] = {false};
+  int dev = 0;
+  L3CI_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    L3CI_CUDA_TRY(cudaFuncSetAttribute(paged_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem(D, kPagedMaxSeqs)));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int parts = cp.p.max_parts;
+  L3CI_LAUNCH("paged_chunk_kernel", paged_chunk_kernel<D>, dim3((unsigned)parts), dim3(kThreads), chunk_smem(D, cp.p.a.B), stream, qmap, kmap, vmap, cp);
+  if (parts > 1) {
+    constexpr int kShares = 2 * kRows * (D / 4) / (kMergeThreads * kMergeItems);
+    L3CI_LAUNCH("paged_chunk_merge_kernel", paged_chunk_merge_kernel<D>, dim3((unsigned)(parts - 1), kShares), dim3(kMergeThreads), 0, stream, cp);
+  }
+  return L3CI_OK;
+}
 
 }  // namespace
 
-size_t paged_chunks_scratch_bytes(const PagedParams& p) { return 0; }
-int paged_chunks_launch(const PagedParams& p, void* scratch, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.a.rows * p.a.Hq + 3) / 4));
-  if (p.a.D == 64) L3CI_LAUNCH("paged_attention_row_kernel", paged_attention_row_kernel<64>, grid, dim3(128), 0, stream, p);
-  else L3CI_LAUNCH("paged_attention_row_kernel", paged_attention_row_kernel<128>, grid, dim3(128), 0, stream, p);
-  return L3CI_OK;
+size_t paged_chunks_scratch_bytes(const PagedParams& p) {
+  const int parts = chunk_parts(p);
+  return (size_t)parts * (sizeof(Cut) + 2 * 4 * (size_t)(p.a.D == 64 ? part_floats<64>() : part_floats<128>()));
+}
+
+int paged_chunks_launch(const PagedParams& params, void* scratch, cudaStream_t stream) {
+  ChunkParams cp = {};
+  cp.p = params;
+  cp.p.max_parts = chunk_parts(params);
+  cp.cuts = static_cast<Cut*>(scratch);
+  cp.p.records = reinterpret_cast<float*>(cp.cuts + cp.p.max_parts);
+  cp.tile_tokens = kRows / params.R;
+  const int low = params.a.page_size & -params.a.page_size;    // tokens that lie together in every page: a power of two
+  cp.box = low < kKeys ? low : kKeys;
+  return params.a.D == 64 ? chunk_launch<64>(cp, stream) : chunk_launch<128>(cp, stream);
 }
 
 }  // namespace l3ci
