@@ -4,6 +4,7 @@
 
 #include "bf16x8.cuh"
 #include "host_common.h"
+#include "linear_rows.h"
 #include "ptx_sm100.cuh"
 #include "warp_reduce.cuh"
 
@@ -12,7 +13,8 @@ namespace {
 
 // z[r, j] = scales[i] x[r] . a[i, j], i = index[r]; 0 without an adapter.  A warp per (r, j).
 __global__ void __launch_bounds__(128) adapter_shrink_kernel(const l3ci_adapter_linear_args p, float* z) {
-  pdl_begin();
+  pdl_wait();                // (before the next kernel may start: it reads x and w at once)
+  pdl_launch_dependents();
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const long long r = item / p.rank;
@@ -105,6 +107,14 @@ extern "C" int l3ci_adapter_linear(const l3ci_adapter_linear_args* a) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
   float* z = static_cast<float*>(a->scratch);
   L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)((a->rows * a->rank + 3) / 4)), dim3(128), 0, stream, *a, z);
+  if (a->rows <= L3CI_LINEAR_MAX_ROWS) {
+    l3ci_linear_args l = {};
+    l.x = a->x; l.w = a->w; l.out = a->out; l.status = a->status;
+    l.rows = a->rows; l.x_st = a->rows > 1 ? a->x_st : a->K; l.out_st = a->out_st;
+    l.K = a->K; l.N = a->N; l.groups = 1;
+    l.stream = a->stream;
+    return adapter_rows_launch(&l, AdapterRows{z, a->index, static_cast<const __nv_bfloat16*>(a->b), a->rank, a->adapters});
+  }
   L3CI_LAUNCH("adapter_expand_kernel", adapter_expand_kernel, dim3((unsigned)((a->N + 63) / 64), (unsigned)((a->rows + 63) / 64)), dim3(256), 0, stream, *a, (const float*)z);
   return L3CI_OK;
 }

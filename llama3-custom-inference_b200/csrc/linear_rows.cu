@@ -24,8 +24,10 @@
 
 #include <type_traits>
 
+#include "bf16x8.cuh"
 #include "host_common.h"
 #include "linear_many.h"
+#include "linear_rows.h"
 #include "mixer_types.cuh"
 #include "ptx_sm100.cuh"
 #include "tcgen05.cuh"
@@ -67,6 +69,7 @@ struct LinParams {
   int group_tiles;                         // tiles of one group
   float limit, alpha;                      // of a gated activation
   l3ci_linear_rope rope;                   // (kernels with ROPE)
+  AdapterRows low;                         // (kernels with ADAPT)
 };
 
 __device__ __forceinline__ float lin_act(float z, int act) {
@@ -108,7 +111,11 @@ __device__ __forceinline__ bool output_warps_agree(bool ok) {
 // ROPE: the outputs are queries, keys and values, which the last step rotates and puts where l3ci_rot_embed_kv_cache_at does, with its
 // bits.  That call took 2.4 us of a layer's 43 at one token and 4001 positions, nearly all of it a launch and a trip to memory each way;
 // here the table and the positions come while the sums still run.  A step of one token 696 -> 668 us.
-template <int NP, int S, int GATE, bool ROPE>
+// ADAPT: every token's low-rank part z b[i]^T (l3ci_adapter_linear) is added to the sums.  The output warps, which have nothing to do while the
+// tensor cores run, compute it in multiply-adds from z in 32 bits, a token after the other: B of the adapters in use is read beside w, a token
+// meets no other's adapter, and nothing waits for it but the stores.  The kernel ahead (adapter_linear.cu) waits for its own predecessors
+// before it lets this one start: w and x may be read at once, and stream while it computes z.
+template <int NP, int S, int GATE, bool ROPE, bool ADAPT>
 __global__ void __launch_bounds__(kThreads, 2)
 linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ LinParams p) {
   using Sh = LinShape<NP>;
@@ -178,6 +185,34 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   };
   Pair pair{};
 
+  // low-rank parts of this thread's outputs: tokens tok0 + i S of column n of a tile
+  constexpr int kMine = ADAPT ? NP / S : 1;
+  float low[kMine];
+  // (numbered by the rows of the accumulator that the warp may read)
+  const int out_thread = (warp & 3) * 32 + lane, tok0 = out_thread / kOwn;
+  float* zs = reinterpret_cast<float*>(tmem_slot + 4);              // [rows][rank], then the rows' adapters
+  auto low_rank = [&](int n) {
+    const AdapterRows& d = p.low;
+    const int* ids = reinterpret_cast<const int*>(zs + (int)a.rows * d.rank);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) low[i] = 0.f;
+    if (n >= a.N) return;
+    for (int r = 0; r < d.rank; r += 8) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int t = tok0 + i * S;
+        if (t >= (int)a.rows) break;
+        const int id = ids[t];
+        if (id < 0) continue;
+        float f[8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(d.b + ((long long)id * a.N + n) * d.rank + r)), f);
+        const float4 z0 = *reinterpret_cast<const float4*>(zs + t * d.rank + r), z1 = *reinterpret_cast<const float4*>(zs + t * d.rank + r + 4);
+        low[i] = fmaf(z0.x, f[0], fmaf(z0.y, f[1], fmaf(z0.z, f[2], fmaf(z0.w, f[3], low[i]))));
+        low[i] = fmaf(z1.x, f[4], fmaf(z1.y, f[5], fmaf(z1.z, f[6], fmaf(z1.w, f[7], low[i]))));
+      }
+    }
+  };
+
   if (warp == 0) {
     // ---- producer ----
     if (lane == 0) {
@@ -200,11 +235,11 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       auto load_x = [&](int s, const At& t) {
         tma_load_4d(ring + s * Sh::kStageBytes + kWBytes, &xmap, full0 + s * 8, (k0 + t.k) * kDeep, 0, 0, t.grp, policy_x);
       };
-      if (!a.early) pdl_wait();
+      if (!ADAPT && !a.early) pdl_wait();
       At w = at_tile(first), x = w;
       int filled = 0;
       for (; filled < kStages && w.tile < p.tiles; ++filled, advance(w)) load_w(filled, w);
-      if (a.early) pdl_wait();
+      if (!ADAPT && a.early) pdl_wait();
       for (int f = 0; f < filled; ++f, advance(x)) load_x(f, x);
       uint32_t parity = 0;
       for (int s = 0; w.tile < p.tiles; advance(w)) {
@@ -217,7 +252,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     ok = __shfl_sync(kFullMask, ok, 0);
   } else if (warp == 1) {
     // ---- MMA issue: all lanes run the code, one elected lane predicates the instructions ----
-    pdl_wait();                          // (the bounds of the waits below count from here, not through the kernels before)
+    if (!ADAPT) pdl_wait();              // (the bounds of the waits below count from here, not through the kernels before)
     constexpr uint32_t idesc = instr_desc(kTile, Sh::kCols, false);
     const uint32_t elected = lane == 0 ? 1u : 0u;
     int s = 0, round = 0;
@@ -242,12 +277,24 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     // ---- output: a thread owns row r of the tile ----
     pdl_wait();
     if constexpr (ROPE) pair = pair_at((int)threadIdx.x - 64);
+    if constexpr (ADAPT) {
+      const int count = (int)a.rows * p.low.rank;
+      int* ids = reinterpret_cast<int*>(zs + count);
+      for (int i = out_thread; i < count / 4; i += 128) reinterpret_cast<float4*>(zs)[i] = __ldcg(reinterpret_cast<const float4*>(p.low.z) + i);
+      for (int i = out_thread; i < (int)a.rows; i += 128) {
+        const int id = __ldg(p.low.index + i);
+        ids[i] = id < p.low.adapters ? id : -1;
+      }
+      output_warps_meet();
+      if constexpr (S > 1) low_rank(first * kOuts + rank * kOwn + out_thread % kOwn);
+    }
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
     const int rows = (int)a.rows;
     int round = 0;
     for (int tile = first; tile < p.tiles; tile += stride, ++round) {
       const int acc = round & 1;
+      if constexpr (ADAPT && S == 1) low_rank(tile * kOuts + out_thread);
       ok = mbar_wait_bounded(done0 + acc * 8, (round >> 1) & 1);
       if (GATED && S == 1) ok = output_warps_agree(ok);
       if (!ok) break;
@@ -277,7 +324,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
           } else if (n < a.N) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (c + i < rows) store_out(a, grp, c + i, n, lin_act(__uint_as_float(v[i]), a.act));
+              if (c + i < rows) store_out(a, grp, c + i, n, ADAPT ? __uint_as_float(v[i]) + low[(c + i) % kMine] : lin_act(__uint_as_float(v[i]), a.act));
           }
         }
         tc_fence_before();
@@ -335,7 +382,20 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
                                                                        turns ? __fmaf_rn(x, sn, __fmul_rn(y, c)) : y);
       }
     }
-    for (int e = threadIdx.x; !ROPE && e < (int)a.rows * kOwn; e += kThreads) {
+    if constexpr (ADAPT) {
+      const int j = out_thread % kOwn, n = first * kOuts + rank * kOwn + j;
+      if (warp >= 2 && n < a.N)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int t = tok0 + i * S;
+          if (t >= (int)a.rows) break;
+          float y = low[i];
+#pragma unroll
+          for (int s = 0; s < S; ++s) y += parts[t * kTile + s * kSlice + j];
+          store_out(a, 0, t, n, y);
+        }
+    }
+    for (int e = threadIdx.x; !ROPE && !ADAPT && e < (int)a.rows * kOwn; e += kThreads) {
       const int t = e / kOwn, j = e % kOwn, n = first % p.group_tiles * kOuts + rank * kOwn + j;
       if (n >= a.N) continue;
       float y = 0.f, u = 0.f;
@@ -356,8 +416,8 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   if (warp == 1) tmem_dealloc(tmem, Sh::kTmem);
 }
 
-template <int NP, int S, int GATE, bool ROPE = false>
-int launch(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t stream, const l3ci_linear_rope* rope = nullptr) {
+template <int NP, int S, int GATE, bool ROPE = false, bool ADAPT = false>
+int launch(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t stream, const l3ci_linear_rope* rope = nullptr, const AdapterRows* low = nullptr) {
   using Sh = LinShape<NP>;
   constexpr bool GATED = GATE > 0;
   constexpr int kOuts = GATED ? kTile / 2 : kTile;
@@ -366,6 +426,8 @@ int launch(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t str
   p.limit = limit;
   p.alpha = alpha;
   if (rope) p.rope = *rope;
+  if (low) p.low = *low;
+  const size_t smem = Sh::kSmem + (low ? (size_t)a->rows * (low->rank + 1) * 4 : 0);
   p.group_tiles = (a->N + kOuts - 1) / kOuts;
   p.tiles = p.group_tiles * a->groups;
   p.steps = (a->K + kDeep - 1) / kDeep;
@@ -373,19 +435,19 @@ int launch(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t str
   CUtensorMap xmap, wmap;
   if (int st = make_rows_map(&xmap, a->x, a->K, (int)a->rows, 1, a->groups, a->x_st, 0, a->x_sg, NP)) return st;
   if (int st = make_rows_map(&wmap, a->w, a->K, a->N, GATED ? 2 : 1, a->groups, a->K, one, one * (GATED ? 2 : 1), kOuts)) return st;
-  auto kernel = linear_rows_kernel<NP, S, GATE, ROPE>;
+  auto kernel = linear_rows_kernel<NP, S, GATE, ROPE, ADAPT>;
   static bool configured[64] = {false};
   int dev = 0;
   L3CI_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    L3CI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::kSmem));
+    L3CI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Sh::kSmem + (ADAPT ? NP * (L3CI_ADAPTER_MAX_RANK + 1) * 4 : 0))));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count() > 0 ? sm_count() : 148;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(S > 1 ? p.tiles * S : p.tiles < 2 * sms ? p.tiles : 2 * sms));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Sh::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -407,18 +469,20 @@ int launch(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t str
   return L3CI_OK;
 }
 
+// The most CTAs that still run at once, two per SM, each with two stages or more (one row, 2048 x 2048: 10.3, 5.9, 4.3, 3.6 us by
+// 1, 2, 4, 8; gated 2 x 8192 x 2048: 13.1, 13.0, 14.8, 20.5; one CTA per SM instead cost a step of the 1B model 40 us).
+int split_for(long long tiles, int K) {
+  const int sms = sm_count() > 0 ? sm_count() : 148, steps = (K + kDeep - 1) / kDeep;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * sms && steps >= 4 * split) split *= 2;
+  return split;
+}
+
 template <int NP, int GATE>
 int launch_split(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t stream) {
   constexpr bool GATED = GATE > 0;
   const long long tiles = (a->N + (GATED ? kTile / 2 : kTile) - 1) / (GATED ? kTile / 2 : kTile) * (long long)a->groups;
-  int split = a->split;
-  if (split == 0) {
-    // the most CTAs that still run at once, two per SM, each with two stages or more (one row, 2048 x 2048: 10.3, 5.9, 4.3, 3.6 us by
-    // 1, 2, 4, 8; gated 2 x 8192 x 2048: 13.1, 13.0, 14.8, 20.5; one CTA per SM instead cost a step of the 1B model 40 us)
-    const int sms = sm_count() > 0 ? sm_count() : 148, steps = (a->K + kDeep - 1) / kDeep;
-    split = 1;
-    while (split < 8 && tiles * split * 2 <= 2 * sms && steps >= 4 * split) split *= 2;
-  }
+  int split = a->split ? a->split : split_for(tiles, a->K);
   while (split > 1 && split > (a->K + kDeep - 1) / kDeep) split /= 2;   // every CTA has a stage
   switch (split) {
     case 1: return launch<NP, 1, GATE>(a, limit, alpha, stream);
@@ -429,7 +493,26 @@ int launch_split(const l3ci_linear_args* a, float limit, float alpha, cudaStream
   }
 }
 
+template <int NP>
+int launch_adapters(const l3ci_linear_args* a, const AdapterRows* low, cudaStream_t stream) {
+  switch (split_for((a->N + kTile - 1) / kTile, a->K)) {
+    case 1: return launch<NP, 1, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
+    case 2: return launch<NP, 2, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
+    case 4: return launch<NP, 4, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
+    default: return launch<NP, 8, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
+  }
+}
+
 }  // namespace
+
+int adapter_rows_launch(const l3ci_linear_args* a, const AdapterRows& low) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
+  if (a->rows <= 8) return launch_adapters<8>(a, &low, stream);
+  if (a->rows <= 16) return launch_adapters<16>(a, &low, stream);
+  if (a->rows <= 32) return launch_adapters<32>(a, &low, stream);
+  return launch_adapters<64>(a, &low, stream);
+}
+
 }  // namespace l3ci
 
 extern "C" int64_t l3ci_row_stride(const int64_t* sizes, const int64_t* strides, int32_t dims) {
