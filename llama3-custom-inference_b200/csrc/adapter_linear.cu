@@ -4,6 +4,7 @@
 
 #include "bf16x8.cuh"
 #include "host_common.h"
+#include "linear_many.h"
 #include "linear_rows.h"
 #include "ptx_sm100.cuh"
 #include "warp_reduce.cuh"
@@ -36,39 +37,93 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const l3ci_adapter_
   if (lane == 0) z[item] = s;
 }
 
-// A tile of 64 x 64 outputs: the shared product and the adapters' part.
-__global__ void __launch_bounds__(256) adapter_expand_kernel(const l3ci_adapter_linear_args p, const float* z) {
-  __shared__ float xs[64][17], ws[64][17];
-  pdl_begin();
-  const long long r0 = (long long)blockIdx.y * 64;
-  const int n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
-      const int y = e >> 4, k = k0 + (e & 15);
-      xs[y][e & 15] = r0 + y < p.rows && k < p.K ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.x)[(r0 + y) * p.x_st + k]) : 0.f;
-      ws[y][e & 15] = n0 + y < p.N && k < p.K ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.w)[(long long)(n0 + y) * p.K + k]) : 0.f;
+// The same of many rows, on the tensor cores: 32 rows of x a CTA, warps share the columns of K and add up at the end.  A dot product does not
+// ask in which order its terms come: a lane takes 8 neighbouring columns, 16 bytes, of a row of x and of a row of a, which are the operands of two
+// products.  Of every adapter among the 32 rows all rows' products are computed and its own rows' kept.
+// CTAs behind these list the adapters among every 256 rows (linear_many.h).
+constexpr int kShrinkRows = 32, kShrinkWarps = 8, kShrinkRanks = 32;   // ranks at a time: four products wide
+
+__global__ void __launch_bounds__(32 * kShrinkWarps) adapter_shrink_many_kernel(const l3ci_adapter_linear_args p, float* z, int* lists, int blocks) {
+  __shared__ float parts[kShrinkWarps][kShrinkRows][kShrinkRanks + 1];
+  __shared__ int ids[kAdapterTile];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  auto id_of = [&](long long row) {
+    const int id = row < p.rows ? __ldg(p.index + row) : -1;
+    return id >= 0 && id < p.adapters ? id : -1;
+  };
+  if ((int)blockIdx.x >= blocks) {       // ---- a list ----
+    const int t = threadIdx.x, tile = blockIdx.x - blocks;
+    ids[t] = id_of((long long)tile * kAdapterTile + t);
+    __syncthreads();
+    bool first = ids[t] >= 0;            // the first row of its adapter
+    for (int i = 0; i < t && first; ++i) first = ids[i] != ids[t];
+    int* counts = reinterpret_cast<int*>(parts);
+    const unsigned mask = __ballot_sync(kFullMask, first);
+    if (lane == 0) counts[warp] = __popc(mask);
+    __syncthreads();
+    int at = __popc(mask & ((1u << lane) - 1)), all = 0;
+    for (int w = 0; w < kShrinkWarps; ++w) {
+      if (w < warp) at += counts[w];
+      all += counts[w];
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[ty * 4 + i][k], ws[tx * 4 + j][k], acc[i][j]);
-    __syncthreads();
+    int* list = lists + (long long)tile * kAdapterList;
+    if (first) list[1 + at] = ids[t];
+    if (t == 0) list[0] = all;
+    return;
   }
+  const long long row0 = (long long)blockIdx.x * kShrinkRows;
+  if (threadIdx.x < kShrinkRows) ids[threadIdx.x] = id_of(row0 + threadIdx.x);
+  __syncthreads();
+  const int mine = ids[lane];
+  unsigned left = __ballot_sync(kFullMask, mine >= 0);     // rows whose adapters are still to come
+  const __nv_bfloat16* x[4];                               // rows gid, gid + 8, + 16, + 24 (the last row for those behind it)
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const long long r = r0 + ty * 4 + i;
-    if (r >= p.rows) break;
-    const int ad = p.index[r];
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx * 4 + j;
-      if (n >= p.N) break;
-      float y = acc[i][j];
-      if (ad >= 0 && ad < p.adapters)
-        for (int k = 0; k < p.rank; ++k) y = fmaf(z[r * p.rank + k], __bfloat162float(static_cast<const __nv_bfloat16*>(p.b)[((long long)ad * p.N + n) * p.rank + k]), y);
-      static_cast<__nv_bfloat16*>(p.out)[r * p.out_st + n] = __float2bfloat16_rn(y);
+    const long long row = row0 + gid + 8 * i;
+    x[i] = static_cast<const __nv_bfloat16*>(p.x) + (row < p.rows ? row : p.rows - 1) * p.x_st + tig * 8;
+  }
+  while (left) {
+    const int id = __shfl_sync(kFullMask, mine, __ffs(left) - 1);
+    const unsigned here = __ballot_sync(kFullMask, mine == id);
+    left &= ~here;
+    const float scale = p.scales ? __ldg(p.scales + id) : 1.f;
+    for (int j0 = 0; j0 < p.rank; j0 += kShrinkRanks) {
+      const int tiles = min(p.rank - j0, kShrinkRanks) / 8;
+      const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + ((long long)id * p.rank + j0 + gid) * p.K + tig * 8;
+      float acc[2][4][4] = {};
+#pragma unroll 2
+      for (int k = warp * 32; k < p.K; k += kShrinkWarps * 32) {
+        const bool in = k + tig * 8 < p.K;                 // (K is a multiple of 8)
+        uint4 xv[4], av[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xv[i] = in ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) av[n] = in && n < tiles ? __ldg(reinterpret_cast<const uint4*>(a + (long long)n * 8 * p.K + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            mma_bf16(acc[m][n], xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y, av[n].x, av[n].y);
+            mma_bf16(acc[m][n], xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w, av[n].z, av[n].w);
+          }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) parts[warp][m * 16 + gid + (e >> 1) * 8][n * 8 + 2 * tig + (e & 1)] = acc[m][n][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < kShrinkRows * tiles * 8; i += 32 * kShrinkWarps) {
+        const int r = i / (tiles * 8), j = i % (tiles * 8);
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kShrinkWarps; ++w) s += parts[w][r][j];
+        if ((here >> r) & 1) z[(row0 + r) * p.rank + j0 + j] = s * scale;
+      }
+      __syncthreads();
     }
   }
 }
@@ -92,29 +147,45 @@ int check(const l3ci_adapter_linear_args* a) {
 }  // namespace
 }  // namespace l3ci
 
+namespace l3ci {
+namespace {
+
+// Scratch: z, then the lists of many rows.
+size_t z_bytes(const l3ci_adapter_linear_args* a) { return ((size_t)a->rows * a->rank * 4 + 15) / 16 * 16; }
+size_t scratch_of(const l3ci_adapter_linear_args* a) {
+  const size_t tiles = ((size_t)a->rows + kAdapterTile - 1) / kAdapterTile;
+  return z_bytes(a) + (a->rows > L3CI_LINEAR_MAX_ROWS ? tiles * kAdapterList * 4 : 0);
+}
+
+}  // namespace
+}  // namespace l3ci
+
 extern "C" size_t l3ci_adapter_linear_scratch_bytes(const l3ci_adapter_linear_args* a) {
   const int st = l3ci::check(a);
   l3ci::clear_error();
-  return st ? 0 : (size_t)a->rows * a->rank * 4;
+  return st ? 0 : l3ci::scratch_of(a);
 }
 
 extern "C" int l3ci_adapter_linear(const l3ci_adapter_linear_args* a) {
   using namespace l3ci;
   clear_error();
   if (int st = check(a)) return st == kNothing ? L3CI_OK : st;
-  const size_t need = (size_t)a->rows * a->rank * 4;
+  const size_t need = scratch_of(a);
   if (!a->scratch || a->scratch_bytes < need || !aligned16(a->scratch)) return fail(L3CI_ERR_SCRATCH, "adapter_linear: %zu bytes of scratch, %zu are needed", a->scratch_bytes, need);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
   float* z = static_cast<float*>(a->scratch);
-  L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)((a->rows * a->rank + 3) / 4)), dim3(128), 0, stream, *a, z);
+  l3ci_linear_args l = {};
+  l.x = a->x; l.w = a->w; l.out = a->out; l.status = a->status;
+  l.rows = a->rows; l.x_st = a->rows > 1 ? a->x_st : a->K; l.out_st = a->out_st;
+  l.K = a->K; l.N = a->N; l.groups = 1;
+  l.stream = a->stream;
+  const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(a->b);
   if (a->rows <= L3CI_LINEAR_MAX_ROWS) {
-    l3ci_linear_args l = {};
-    l.x = a->x; l.w = a->w; l.out = a->out; l.status = a->status;
-    l.rows = a->rows; l.x_st = a->rows > 1 ? a->x_st : a->K; l.out_st = a->out_st;
-    l.K = a->K; l.N = a->N; l.groups = 1;
-    l.stream = a->stream;
-    return adapter_rows_launch(&l, AdapterRows{z, a->index, static_cast<const __nv_bfloat16*>(a->b), a->rank, a->adapters});
+    L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)((a->rows * a->rank + 3) / 4)), dim3(128), 0, stream, *a, z);
+    return adapter_rows_launch(&l, AdapterRows{z, a->index, b, a->rank, a->adapters});
   }
-  L3CI_LAUNCH("adapter_expand_kernel", adapter_expand_kernel, dim3((unsigned)((a->N + 63) / 64), (unsigned)((a->rows + 63) / 64)), dim3(256), 0, stream, *a, (const float*)z);
-  return L3CI_OK;
+  int* lists = reinterpret_cast<int*>(static_cast<uint8_t*>(a->scratch) + z_bytes(a));
+  const long long blocks = (a->rows + kShrinkRows - 1) / kShrinkRows, tiles = (a->rows + kAdapterTile - 1) / kAdapterTile;
+  L3CI_LAUNCH("adapter_shrink_many_kernel", adapter_shrink_many_kernel, dim3((unsigned)(blocks + tiles)), dim3(32 * kShrinkWarps), 0, stream, *a, z, lists, (int)blocks);
+  return adapter_many_launch(&l, AdapterMany{z, a->index, b, lists, a->rank, a->adapters});
 }

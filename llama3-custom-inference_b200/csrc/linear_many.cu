@@ -37,6 +37,8 @@ constexpr int kPieceCols = 32;             // columns that a group takes at a ti
 constexpr int kPieceBytes = kHalf * kPieceCols * 2;
 constexpr int kThreads = 32 * (4 + kOutWarps);   // producer, MMA issue, allocation, none; outputs
 constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kBox + kOutWarps / 4 * kPieceBytes;
+constexpr size_t kAdaptSmem = kSmem + 2 * kBox;   // with the two boxes of z
+constexpr int kMarks = 4;                  // tiles with adapters whose marks are kept: the filling warps are at most three of them ahead of the output warps
 
 __device__ int g_wait_status = 0;
 
@@ -45,6 +47,7 @@ struct ManyParams {
   int steps, N, rows;
   __nv_bfloat16* out;
   long long out_st;
+  AdapterMany low;                         // (kernels with ADAPT)
 };
 
 typedef unsigned long long f2;             // two floats
@@ -117,17 +120,32 @@ __device__ __forceinline__ float silu_mul(float z, float u) {
   return bf16_of(__fdividef(z * 0.0625f, fmaf(__expf(-z), 0.0625f, 0.0625f))) * bf16_of(u);
 }
 
-template <int ACT>
+__device__ __forceinline__ bool no_numbers(const uint4& v) {   // a bf16 that is NaN or infinite among eight
+  auto any = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+  return any(v.x) || any(v.y) || any(v.z) || any(v.w);
+}
+
+// ADAPT: low-rank parts beside the product (l3ci_adapter_linear), as further columns: behind a tile's K columns come, for every adapter among its
+// 256 rows, the adapter's b as w and its rows' z as x, zeros in the rows of others, so that the parts land in the same accumulator and
+// are rounded once with it.  z is fp32: it goes in as two bf16 that add up to 2^-17 of it.  The boxes of z are written by two warps of each CTA
+// (while the K columns run).  0 times what is no number is none: an adapter whose b holds such values in the tile's columns is left out,
+// and its rows' parts are added by the output warps in multiply-adds.
+template <int ACT, bool ADAPT>
 __global__ void __launch_bounds__(kThreads, 1)
-linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ ManyParams p) {
+linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap bmap,
+                   const __grid_constant__ ManyParams p) {
   constexpr bool GATED = ACT == L3CI_ACT_SILU_GATE || ACT == L3CI_ACT_SILU_MUL;
   constexpr int kOuts = GATED ? kHalf : 2 * kHalf;       // output columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* out_box = smem + kStages * 2 * kBox;
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
+  const uint32_t z_box = smem_u32(smem + kSmem - 1024);            // ADAPT: the upper halves of z, then what they leave
+  __shared__ uint8_t marks[ADAPT ? kMarks : 1][kHalf];             // ADAPT: rows whose parts are the output warps'
+  __shared__ int left_out;                                         // ADAPT: the filled boxes are not to be multiplied
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 6];
   __shared__ uint32_t tmem_slot;
-  const uint32_t ring = smem_u32(smem), full0 = smem_u32(bars), empty0 = full0 + kStages * 8, done0 = empty0 + kStages * 8, read0 = done0 + 16;
+  const uint32_t ring = smem_u32(smem), full0 = smem_u32(bars), empty0 = full0 + kStages * 8, done0 = empty0 + kStages * 8, read0 = done0 + 16,
+                 z_full = read0 + 16, z_empty = z_full + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const long long pair = blockIdx.x / 2, pairs = gridDim.x / 2;
@@ -141,6 +159,8 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       mbar_init(done0 + i * 8, 1);
       mbar_init(read0 + i * 8, 2 * kOutWarps);
     }
+    mbar_init(z_full, 4);
+    mbar_init(z_empty, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -155,6 +175,8 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   const uint32_t tmem = tmem_slot;
   pdl_launch_dependents();
   pdl_wait();
+  const int chunks = ADAPT ? (p.low.rank + kDeep - 1) / kDeep : 0;             // columns of z of one adapter, 64 at a time
+  auto list_of = [&](long long tile) { return p.low.lists + tile % p.m_tiles * kAdapterList; };   // number, then the adapters among a tile's rows
   bool ok = true;
   int asked = 0;
 
@@ -175,6 +197,16 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
           pair_load(dst + kBox, &wmap, bar, k * kDeep, col, GATED ? (int)rank : 0);
           if (++s == kStages) { s = 0; parity ^= 1; }
         }
+        if constexpr (ADAPT) {
+          const int* list = list_of(tile);
+          for (int i = 0; i < list[0] * chunks && ok; ++i) {
+            if (!mbar_wait_bounded_one(empty0 + s * 8, parity)) { ok = false; break; }
+            ++asked;
+            if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * kBox);
+            pair_load(ring + s * 2 * kBox + kBox, &bmap, first_cta(full0 + s * 8), i % chunks * kDeep, col, list[1 + i / chunks]);
+            if (++s == kStages) { s = 0; parity ^= 1; }
+          }
+        }
       }
       // (the stages' last arrivals come from the pair's products: this CTA must not leave ahead of them)
       for (int i = 0; i < kStages && i < asked && ok; ++i) {
@@ -188,7 +220,7 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     // ---- MMA issue, for both: all lanes run the code, one elected lane predicates the instructions ----
     constexpr uint32_t idesc = instr_desc(2 * kHalf, kCols, false);
     const uint32_t elected = lane == 0 ? 1u : 0u;
-    int s = 0, round = 0;
+    int s = 0, round = 0, filled = 0;
     uint32_t parity = 0;
     for (long long tile = pair; tile < p.tiles && ok; tile += pairs, ++round) {
       const int acc = round & 1;
@@ -203,8 +235,83 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         pair_commit(empty0 + s * 8, elected);
         if (++s == kStages) { s = 0; parity ^= 1; }
       }
+      if constexpr (ADAPT) {
+        const int count = ok ? list_of(tile)[0] * chunks : 0;
+        for (int i = 0; i < count; ++i, ++filled) {
+          if (!mbar_wait_bounded(full0 + s * 8, parity) || !mbar_wait_bounded(z_full, filled & 1)) { ok = false; break; }
+          tc_fence_after();
+          if (!*reinterpret_cast<volatile int*>(&left_out)) {
+            const uint64_t zd = smem_desc(z_box, 16, 1024), ld = smem_desc(z_box + kBox, 16, 1024), bd = smem_desc(ring + s * 2 * kBox + kBox, 16, 1024);
+            const int steps = (min(p.low.rank - i % chunks * kDeep, kDeep) + 15) / 16;
+            for (int k = 0; k < steps; ++k) pair_mma(tmem + acc * kCols, zd + k * 2, bd + k * 2, idesc, 1u, elected);
+            for (int k = 0; k < steps; ++k) pair_mma(tmem + acc * kCols, ld + k * 2, bd + k * 2, idesc, 1u, elected);
+          }
+          pair_commit(empty0 + s * 8, elected);
+          pair_commit(z_empty, elected);
+          if (++s == kStages) { s = 0; parity ^= 1; }
+        }
+      }
       if (ok) pair_commit(done0 + acc * 8, elected);
     }
+  } else if (ADAPT && (warp == 2 || warp == 3)) {
+    // ---- ADAPT: boxes of z, two rows a lane ----
+    const AdapterMany& d = p.low;
+    int listed = 0, filled = 0;          // tiles with adapters, boxes
+    for (long long tile = pair; tile < p.tiles && ok; tile += pairs) {
+      const int row0 = (int)(tile % p.m_tiles) * 2 * kHalf + (int)rank * kHalf, col = (int)(tile / p.m_tiles) * kOuts;
+      const int* list = list_of(tile);
+      if (list[0] == 0) continue;
+      uint8_t* mark = marks[listed++ % kMarks];
+      const int r[2] = {(warp - 2) * 64 + lane, (warp - 2) * 64 + 32 + lane};
+      int id[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        id[i] = row0 + r[i] < p.rows ? __ldg(d.index + row0 + r[i]) : -1;
+        mark[r[i]] = 0;
+      }
+      for (int a = 0; a < list[0] && ok; ++a) {
+        const int adapter = list[1 + a];
+        // (the columns of both CTAs, so that both decide alike)
+        const uint4* b = reinterpret_cast<const uint4*>(d.b + ((long long)adapter * p.N + col) * d.rank);
+        const int vecs = min(2 * kHalf, p.N - col) * (d.rank / 8);
+        bool odd = false;
+#pragma unroll 4
+        for (int v = lane; v < vecs; v += 32) odd |= no_numbers(__ldg(b + v));
+        odd = __any_sync(kFullMask, odd);
+        for (int c = 0; c < chunks; ++c, ++filled) {
+          if (filled > 0 && !mbar_wait_bounded(z_empty, (filled - 1) & 1)) { ok = false; break; }
+          const int wide = min(d.rank - c * kDeep, kDeep);
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            const bool mine = id[i] == adapter && !odd;
+            if (id[i] == adapter && odd) mark[r[i]] = 1;
+            const float4* z = reinterpret_cast<const float4*>(d.z + (long long)(row0 + r[i]) * d.rank + c * kDeep);
+#pragma unroll 2
+            for (int v = 0; v < kDeep / 8; ++v) {
+              uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+              if (mine && v * 8 < wide) {
+                const float4 f0 = __ldg(z + 2 * v), f1 = __ldg(z + 2 * v + 1);
+                float f[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w}, h[8];
+                hi = pack8(f);
+                unpack8(hi, h);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = fabsf(h[e]) < INFINITY ? f[e] - h[e] : 0.f;   // (what is no number goes in once)
+                lo = pack8(f);
+              }
+              const uint32_t at = z_box + r[i] * 128 + ((v ^ (r[i] & 7)) << 4);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + kBox), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+            }
+          }
+          if (warp == 2 && lane == 0) left_out = odd;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_cluster(first_cta(z_full));
+        }
+      }
+    }
+    // (the last arrival on z_empty comes from the pair's products: this CTA must not leave ahead of it)
+    if (ok && filled > 0 && !mbar_wait_bounded(z_empty, (filled - 1) & 1)) ok = false;
   } else if (warp >= 4) {
     // ---- outputs: a thread owns a row; each group of four warps takes a quarter of the columns, 32 at a time through its box ----
     const int q4 = warp & 3, part = (warp - 4) >> 2, r = q4 * 32 + lane;
@@ -212,7 +319,7 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     uint8_t* box = out_box + part * kPieceBytes;
     constexpr int kShare = kOuts / (kOutWarps / 4);
     auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory"); };
-    int round = 0;
+    int round = 0, listed = 0;
     for (long long tile = pair; tile < p.tiles && ok; tile += pairs, ++round) {
       const int acc = round & 1;
       const int row = (int)(tile % p.m_tiles) * 2 * kHalf + (int)rank * kHalf, col = (int)(tile / p.m_tiles) * kOuts;
@@ -224,6 +331,9 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       }
       if (!ok) break;
       tc_fence_after();
+      bool marked = false;                     // (the filling warps have written the marks ahead of the boxes that the products waited for)
+      if constexpr (ADAPT)
+        if (list_of(tile)[0] > 0) marked = *const_cast<volatile uint8_t*>(&marks[listed++ % kMarks][r]) != 0;
 #pragma unroll 1
       for (int c0 = part * kShare; c0 < (part + 1) * kShare; c0 += kPieceCols) {
         meet();                                // the box has been read
@@ -244,6 +354,17 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
               else if (GATED) f[i] = gated_activation(f[i], __uint_as_float(z[v * 8 + i]), 0.f, 0.f);
               else if (ACT == L3CI_ACT_TANH) f[i] = tanhf(f[i]);
             }
+            if (marked)                        // (z b of a row whose adapter was left out)
+              for (int i = 0; i < 8; ++i) {
+                const int n = col + c0 + c + v * 8 + i;
+                if (n >= p.N) break;
+                const float* z = p.low.z + (long long)(row + r) * p.low.rank;
+                const __nv_bfloat16* b = p.low.b + ((long long)__ldg(p.low.index + row + r) * p.N + n) * p.low.rank;
+                float y = 0.f;
+                for (int k = 0; k < p.low.rank; ++k) y = fmaf(__ldg(z + k), __bfloat162float(b[k]), y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] += e == i ? y : 0.f;
+              }
             if (ACT == L3CI_ACT_GELU)
 #pragma unroll
               for (int i = 0; i < 8; i += 2) gelu(f[i], f[i + 1]);
@@ -277,8 +398,8 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kCols) : "memory");
 }
 
-template <int ACT>
-int launch(const l3ci_linear_args* a) {
+template <int ACT, bool ADAPT = false>
+int launch(const l3ci_linear_args* a, const AdapterMany* low = nullptr) {
   constexpr bool GATED = ACT == L3CI_ACT_SILU_GATE || ACT == L3CI_ACT_SILU_MUL;
   ManyParams p = {};
   const int outs = GATED ? kHalf : 2 * kHalf;
@@ -287,25 +408,31 @@ int launch(const l3ci_linear_args* a) {
   p.steps = (a->K + kDeep - 1) / kDeep;
   p.N = a->N;
   const long long one = (long long)a->N * a->K;
-  CUtensorMap xmap, wmap;
+  CUtensorMap xmap, wmap, bmap = {};
+  if (low) {
+    p.low = *low;
+    if (low->adapters > 0)
+      if (int st = make_rows_map(&bmap, low->b, low->rank, a->N, low->adapters, 1, low->rank, (long long)a->N * low->rank, 0, kHalf)) return st;
+  }
+  constexpr size_t smem = ADAPT ? kAdaptSmem : kSmem;
   if (int st = make_rows_map(&xmap, a->x, a->K, (int)a->rows, 1, 1, a->x_st, 0, 0, kHalf)) return st;
   if (int st = make_rows_map(&wmap, a->w, a->K, a->N, GATED ? 2 : 1, 1, a->K, one, one * 2, kHalf)) return st;
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.out_st = a->rows > 1 ? a->out_st : a->N;
   p.rows = (int)a->rows;
-  auto kernel = linear_many_kernel<ACT>;
+  auto kernel = linear_many_kernel<ACT, ADAPT>;
   static bool configured[64] = {false};
   int dev = 0;
   L3CI_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    L3CI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    L3CI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count() > 0 ? sm_count() : 148;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * (p.tiles < sms / 2 ? p.tiles : sms / 2)));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = reinterpret_cast<cudaStream_t>(a->stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -315,12 +442,14 @@ int launch(const l3ci_linear_args* a) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = programmatic_launch_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, xmap, wmap, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, xmap, wmap, bmap, p);
   if (e != cudaSuccess) return fail(L3CI_ERR_CUDA, "launch of linear_many_kernel failed: %s", cudaGetErrorString(e));
   return L3CI_OK;
 }
 
 }  // namespace
+
+int adapter_many_launch(const l3ci_linear_args* a, const AdapterMany& low) { return launch<L3CI_ACT_NONE, true>(a, &low); }
 
 int* linear_many_wait_status() {
   void* at = nullptr;

@@ -19,11 +19,12 @@ def make(device, rows, K, N, rank, adapters, index, seed=0):
                 scales=(0.5 + torch.rand(adapters, generator=g)).to(device))
 
 
-def check(got, c):
+def check(got, c, rows=slice(None), columns=slice(None)):
     want, size, low = paged.adapter_linear(c["x"].reshape(-1, c["x"].shape[-1]), c["w"], c["a"], c["b"], c["index"].cpu().view(-1), c.get("scales"))
     K, rank = c["x"].shape[-1], c["a"].shape[1]
     off = (got.reshape(want.shape).double() - want).abs()
     bound = want.abs() * 2 ** -8 + size * K * 2 ** -23 + low * ((K + rank) * 2 ** -23 + 2 ** -16)
+    off, bound = off[rows][:, columns], bound[rows][:, columns]
     assert bool((off <= bound).all()), f"{(off / bound).max().item():.3g} of the bound"
 
 
@@ -79,7 +80,9 @@ def test_an_adapter_that_is_no_number_stays_with_its_rows(ext, device, rows):
     assert torch.equal(got[0::3], clean[0::3]) and torch.isnan(got[1::3]).all()
     third = torch.ones(128, dtype=torch.bool, device=device)
     third[7] = False
-    assert torch.equal(got[2::3][:, third], clean[2::3][:, third]) and not torch.isfinite(got[2::3][:, 7]).any()
+    # its own rows may be summed in another order then (multiply-adds for tensor cores): any order is within the bound, the bits may differ
+    check(got, c, slice(2, None, 3), third)
+    assert not torch.isfinite(got[2::3][:, 7]).any()
 
 
 def test_shapes_strides_and_default_scales(ext, device):
