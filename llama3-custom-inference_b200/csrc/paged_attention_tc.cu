@@ -39,6 +39,7 @@ static_assert(4 * kRegsLow + kSoftmaxWarps * kRegsHigh + 4 * kRegsOut <= 16 * 12
 constexpr uint32_t kTmemCols = 512;                            // S_0, S_1 (128 columns each), O_0, O_1 (D columns each)
 constexpr int kMarks = 4;      // the guards are at most three segments ahead of the output (one-tile segments: two in the ring of V, one on its way out)
 constexpr int kMergeThreads = 256;
+constexpr int kUnitCost = 1;                                   // columns that a unit counts beside its tiles: its start and its end
 constexpr int kMergeItems = 4;                                 // float4 a thread merges
 
 // The unit that part g of the deal begins in the middle of, written by its CTA for the merge; parts 0: none, or its first cut is another part's.
@@ -68,6 +69,11 @@ __device__ __forceinline__ int unit_tiles(const PagedSeq& s, int m, int block) {
   return seen <= 0 ? 1 : (seen + kKeys - 1) / kKeys;
 }
 
+// A run of keys' tiles of a unit; first: the unit's first column.
+struct Unit {
+  int b, h, m, n, len, first, tiles;
+};
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -85,20 +91,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const uint32_t v_smem = k_smem + kStages * kTileBytes;       // [kStages]
   uint8_t* stage_all = smem + (2 + 2 * kStages) * kTileBytes;  // [2 tiles][128 rows][kSPitch]
   uint64_t* bars = reinterpret_cast<uint64_t*>(stage_all + 2 * kRows * kSPitch);
-  // as in prefill_tc_persist_kernel; V_GO: the guard warps may go through a tile of V, which has landed; V_OK: they have
-  enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_GO = 14, V_OK = 15, P_FULL = 16, L_FULL = 18, O_READ = 20,
+  // as in prefill_tc_persist_kernel; V_OK: the guard warps have been through the tile, if it is one of theirs
+  // (they arrive on V_EMPTY too, so that they never miss a phase of V_FULL)
+  enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_OK = 14, P_FULL = 16, L_FULL = 18, O_READ = 20,
          N_BARS = 22 };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
   int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kMarks]: values taken out of tiles of a segment
   int* sums = odd + kMarks;                                            // [16 warps]
   float* stat = reinterpret_cast<float*>(sums + 16);               // [2 tiles][128 rows][l, m_ref]
-  int* pref = reinterpret_cast<int*>(stat + 4 * kRows);            // [B + 1]
+  Unit* units = reinterpret_cast<Unit*>(stat + 4 * kRows);         // [16 warps]: where each is (registers are few)
+  int* pref = reinterpret_cast<int*>(units + 16);                  // [B + 1]
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_FULL ? kSoftmaxWarps / 2 : i == V_OK ? 2 : 1);
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_FULL ? kSoftmaxWarps / 2 : i >= V_OK ? 2 : i == V_EMPTY || i == V_EMPTY + 1 ? 3 : 1);
     for (int i = 0; i < kMarks; ++i) odd[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -111,11 +119,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     tmem_relinquish();
   }
   pdl_wait();
-  // ---- columns (a unit's tile of keys each) before every sequence ----
+  // ---- columns (kUnitCost and a tile of keys each of every unit) before every sequence ----
   const int block = 2 * cp.tile_tokens;
   auto columns_of_head = [&](const PagedSeq& s) {
     int sum = 0;
-    for (int m = 0; m * block < s.n; ++m) sum += unit_tiles(s, m, block);
+    for (int m = 0; m * block < s.n; ++m) sum += kUnitCost + unit_tiles(s, m, block);
     return sum;
   };
   {
@@ -150,7 +158,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const int begin = part < parts ? fd_range_begin(part, total, parts) : 0, end = part < parts ? fd_range_begin(part + 1, total, parts) : 0;
 
   // ---- a CTA's run is a list of segments: tiles [j0, j1) of a unit ----
-  struct Unit { int b, h, m, n, len, first, tiles; };   // first: its first column
   auto unit_at = [&](int col) {                         // the unit that holds a column
     int lo = 0, hi = a.B;
     while (hi - lo > 1) {
@@ -167,14 +174,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     int before = u.h * per_head;
     for (u.m = 0;; ++u.m) {
       u.tiles = unit_tiles(s, u.m, block);
-      if (before + u.tiles > local) break;
-      before += u.tiles;
+      if (before + kUnitCost + u.tiles > local) break;
+      before += kUnitCost + u.tiles;
     }
     u.first = pref[lo] + before;
     return u;
   };
   auto next_unit = [&](Unit& u) {
-    u.first += u.tiles;
+    u.first += kUnitCost + u.tiles;
     if (++u.m * block >= u.n) {
       u.m = 0;
       if (++u.h == a.Hkv) {
@@ -188,13 +195,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
     u.tiles = unit_tiles(PagedSeq{u.n, u.len}, u.m, block);
   };
-  auto tiles_from = [&](const Unit& u, int col) { return col - u.first; };
-  auto tiles_to = [&](const Unit& u) { return min(u.tiles, end - u.first); };
+  auto tiles_from = [&](const Unit& u, int col) { return max(col - u.first - kUnitCost, 0); };
+  auto tiles_to = [&](const Unit& u) { return max(min(u.tiles, end - u.first - kUnitCost), 0); };
+  // to the unit behind u, whose tiles up to j1 have been dealt with; false: the run ends
+  auto next_segment = [&](Unit& u, int j1) {
+    if (j1 < u.tiles) return false;
+    next_unit(u);
+    return u.first + kUnitCost < end;
+  };
   auto both = [&](const Unit& u) { return u.m * block + cp.tile_tokens < u.n; };      // the second tile of rows has tokens
   auto first_limit = [&](const Unit& u, int e) { return u.len - u.n + u.m * block + e * cp.tile_tokens; };   // last key of the tile's first token
   auto cut_tile = [&](int j, int limit) { return j * kKeys + kKeys - 1 > limit; };    // some row does not see all keys
   bool ok = true;
   int fill = 0;        // tiles of keys so far: stage and phase of the rings follow
+  Unit& u = units[warp];
+  u = begin < end ? unit_at(begin) : Unit{};
+  bool on = tiles_to(u) > tiles_from(u, begin);   // there is something to do
   int segments = 0;
 
   if (warp == 0) {
@@ -202,48 +218,45 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     // ---- producer: lane 0 the query rows, every lane the tokens of its own copies ----
     const uint64_t policy = l2_evict_first_policy();
     const int copies = kKeys / cp.box;                      // per half of a tile
-    Unit u = begin < end ? unit_at(begin) : Unit{};
-    for (int col = begin; col < end && ok; ++segments) {
-      if (segments > 0 && !mbar_wait_bounded(bar(Q_EMPTY), (segments - 1) & 1)) { ok = false; break; }
-      const int t0 = u.m * block;
-      if (lane == 0) {
-        const int tiles = both(u) ? 2 : 1, rows = cp.tile_tokens * p.R;
-        const int row = a.starts ? __ldg(a.starts + u.b) + t0 : t0;
-        mbar_expect_tx(bar(Q_FULL), tiles * kHalves * rows * 128);
-        for (int e = 0; e < tiles; ++e)
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_load_4d(q_smem + e * kTileBytes + h * kBoxBytes, &qmap, bar(Q_FULL), h * 64, u.h * p.R, row + e * cp.tile_tokens, a.starts ? 0 : u.b, policy);
-      }
+    for (int col = begin; on && ok; ++segments) {
       auto page_of = [&](int j) {                          // of this lane's tokens of tile j; one past the last: nothing is there
         const int token = j * kKeys + lane * cp.box;
         const int page = lane < copies && token < u.len ? __ldg(a.page_table + u.b * a.table_st + token / a.page_size) : -1;
         return page >= 0 && page < a.pages ? page : (int)a.pages;
       };
-      const int j1 = tiles_to(u);
-      int j = tiles_from(u, col), page = page_of(j);
-      for (; j < j1 && ok; ++j, ++fill) {
+      const int j0 = tiles_from(u, col), j1 = tiles_to(u);
+      const int row = (a.starts ? __ldg(a.starts + u.b) : 0) + u.m * block;
+      int page = page_of(j0);
+      for (int j = j0; j < j1 && ok; ++j, ++fill) {
         const int s = fill % kStages, off = (j * kKeys + lane * cp.box) % a.page_size;
         const int ahead = page_of(j + 1);
         const uint32_t par = ((fill / kStages) - 1) & 1;
+        auto load = [&](const CUtensorMap& map, uint32_t to, uint32_t full) {
+          if (lane == 0) mbar_expect_tx(full, kTileBytes);
+          __syncwarp();
+          if (lane < copies)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) tma_load_4d(to + s * kTileBytes + h * kBoxBytes + lane * cp.box * 128, &map, full, h * 64, off, u.h, page, policy);
+        };
         if (fill >= kStages && !mbar_wait_bounded(bar(K_EMPTY + s), par)) { ok = false; break; }
-        if (lane == 0) mbar_expect_tx(bar(K_FULL + s), kTileBytes);
-        __syncwarp();
-        if (lane < copies)
+        load(kmap, k_smem, bar(K_FULL + s));
+        if (j == j0) {     // (behind the first keys, whose place is free before the last unit's scores are done)
+          if (segments > 0 && !mbar_wait_bounded(bar(Q_EMPTY), (segments - 1) & 1)) { ok = false; break; }
+          if (lane == 0) {
+            const int tiles = both(u) ? 2 : 1;
+            mbar_expect_tx(bar(Q_FULL), tiles * kHalves * cp.tile_tokens * p.R * 128);
+            for (int e = 0; e < tiles; ++e)
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_load_4d(k_smem + s * kTileBytes + h * kBoxBytes + lane * cp.box * 128, &kmap, bar(K_FULL + s), h * 64, off, u.h, page, policy);
+              for (int h = 0; h < kHalves; ++h)
+                tma_load_4d(q_smem + e * kTileBytes + h * kBoxBytes, &qmap, bar(Q_FULL), h * 64, u.h * p.R, row + e * cp.tile_tokens, a.starts ? 0 : u.b, policy);
+          }
+        }
         if (fill >= kStages && !mbar_wait_bounded(bar(V_EMPTY + s), par)) { ok = false; break; }
-        if (lane == 0) mbar_expect_tx(bar(V_FULL + s), kTileBytes);
-        __syncwarp();
-        if (lane < copies)
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_load_4d(v_smem + s * kTileBytes + h * kBoxBytes + lane * cp.box * 128, &vmap, bar(V_FULL + s), h * 64, off, u.h, page, policy);
+        load(vmap, v_smem, bar(V_FULL + s));
         page = ahead;
       }
-      col = u.first + j1;
-      if (col < end) next_unit(u);
+      on = next_segment(u, j1);
+      col = u.first;
     }
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
@@ -251,112 +264,131 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     constexpr uint32_t idesc_qk = instr_desc(kRows, kKeys, false);
     constexpr uint32_t idesc_pv = instr_desc(kRows, D, true);
     const uint32_t elected = lane == 0 ? 1u : 0u;
-    const uint64_t q_desc = smem_desc(q_smem, 16, 1024);
-    const uint64_t k_desc = smem_desc(k_smem, 16, 1024);
-    const uint64_t v_desc = smem_desc(v_smem, kBoxBytes, 1024);
-    // S_{e,g} = Q_e K^T (g: tile number over all segments) into tile e's score accumulator
-    auto issue_s = [&](int e, int g, bool last_of_tile, bool last_of_segment) {
-      const int s = g % kStages;
-      const uint64_t qd = q_desc + (uint64_t)((e * kTileBytes) >> 4);
-      const uint64_t kd = k_desc + (uint64_t)((s * kTileBytes) >> 4);
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint64_t step = (uint64_t)(((ks >> 2) * kBoxBytes + (ks & 3) * 32) / 16);
-        mma_ss(t_s[e], qd + step, kd + step, idesc_qk, ks > 0, elected);
-      }
-      tc_commit(bar(S_FULL + e), elected);
-      if (last_of_tile) {
-        tc_commit(bar(K_EMPTY + s), elected);
-        if (last_of_segment) tc_commit(bar(Q_EMPTY), elected);
-      }
-    };
-    int done[2] = {0, 0}, seg_of[2] = {0, 0};   // tiles and segments of each tile of rows
-    int guarded = 0;                          // tiles that the guards have been through
-    Unit u = begin < end ? unit_at(begin) : Unit{};
-    for (int col = begin; col < end && ok; ++segments) {
-      const int j0 = tiles_from(u, col), j1 = tiles_to(u), ne = both(u) ? 2 : 1, limit = first_limit(u, 0);
-      if (!mbar_wait_bounded(bar(Q_FULL), segments & 1)) { ok = false; break; }
-      if (!mbar_wait_bounded(bar(K_FULL + fill % kStages), (fill / kStages) & 1)) { ok = false; break; }
-      tc_fence_after();
-      for (int e = 0; e < ne; ++e) issue_s(e, fill, e == ne - 1, j0 + 1 == j1);
-      for (int j = j0; j < j1 && ok; ++j, ++fill) {
-        const int s = fill % kStages;
+    // the lower halves of the operands' descriptors; the upper ones are all alike
+    const uint32_t q_desc = (uint32_t)smem_desc(q_smem, 16, 1024), k_desc = (uint32_t)smem_desc(k_smem, 16, 1024), v_desc = (uint32_t)smem_desc(v_smem, kBoxBytes, 1024);
+    auto desc = [](uint32_t low) { return (uint64_t)low | (smem_desc(0, 0, 1024) & 0xffffffff00000000ull); };
+    // One loop over the tiles of all segments, a round ahead with the scores: a unit's first scores follow the last product of the one before at
+    // once, and there is one place for each product's code (what is unrolled further falls out of the instruction cache that the warp shares with
+    // the softmax: with both tiles of rows and both stages unrolled a tile of keys took 3.3 us instead of 2.7).
+    uint32_t p_phase = 0, o_phase = 0, o_used = 0, guarded = 0;   // phases of P_FULL, O_READ and V_OK, a bit for each; whether O_e has been used
+    int nj = tiles_from(u, begin), nj1 = tiles_to(u), nne = both(u) ? 2 : 1, nlimit = first_limit(u, 0);   // the tile whose scores come
+    int j = 0, ne = 0, limit = 0;                                 // the tile whose values come: the one before; ne 0: none
+    bool first = true, nfirst = true;
+    for (fill = -1; (on || ne > 0) && ok; ++fill) {
+      const int s = fill & (kStages - 1), ns = (fill + 1) & (kStages - 1);
+      if (ne > 0) {
         if (!mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
-        bool guard = false;
         if (cut_tile(j, limit)) {
-          if (lane == 0) mbar_arrive(bar(V_GO));
-          guard = true;
+          if (!mbar_wait_bounded(bar(V_OK + s), (guarded >> s) & 1)) { ok = false; break; }
+          guarded ^= 1u << s;
         }
-        for (int e = 0; e < ne; ++e) {
+      }
+#pragma unroll 1
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t s_at = tmem + 128u * e, o_at = tmem + 256u + (uint32_t)D * e;
+        if (e < ne) {
           // O_e += P_e V once P_e is in tensor memory, on a segment's first tile once the last segment's O_e has been read; then at
           // once the next scores, which go where P_e lay
-          if (!mbar_wait_bounded(bar(P_FULL + e), done[e] & 1)) { ok = false; break; }
-          if (j == j0 && seg_of[e] > 0 && !mbar_wait_bounded(bar(O_READ + e), (seg_of[e] - 1) & 1)) { ok = false; break; }
-          if (guard) {
-            if (!mbar_wait_bounded(bar(V_OK), guarded & 1)) { ok = false; break; }
-            ++guarded;
-            guard = false;
+          if (!mbar_wait_bounded(bar(P_FULL + e), (p_phase >> e) & 1)) { ok = false; break; }
+          p_phase ^= 1u << e;
+          if (first) {
+            if ((o_used >> e) & 1) {
+              if (!mbar_wait_bounded(bar(O_READ + e), (o_phase >> e) & 1)) { ok = false; break; }
+              o_phase ^= 1u << e;
+            }
+            o_used |= 1u << e;
           }
           tc_fence_after();
-          const uint64_t vd = v_desc + (uint64_t)((s * kTileBytes) >> 4);
+          const uint32_t vd = v_desc + s * (kTileBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_ts(t_o[e], t_s[e] + kk * 8, vd + (uint64_t)(kk * 128), idesc_pv, (j > j0 || kk > 0) ? 1u : 0u, elected);
+          for (int kk = 0; kk < kKeys / 16; ++kk) mma_ts(o_at, s_at + kk * 8, desc(vd + kk * 128), idesc_pv, (!first || kk > 0) ? 1u : 0u, elected);
           tc_commit(bar(O_FULL + e), elected);
           if (e == ne - 1) tc_commit(bar(V_EMPTY + s), elected);
-          ++done[e];
-          if (j + 1 < j1) {
-            if (e == 0) {
-              if (!mbar_wait_bounded(bar(K_FULL + (fill + 1) % kStages), ((fill + 1) / kStages) & 1)) { ok = false; break; }
-              tc_fence_after();
-            }
-            issue_s(e, fill + 1, e == ne - 1, j + 2 == j1);
+        }
+        if (on && e < nne) {
+          if (e == 0) {
+            if (!mbar_wait_bounded(bar(K_FULL + ns), ((fill + 1) / kStages) & 1)) { ok = false; break; }
+            if (nfirst && !mbar_wait_bounded(bar(Q_FULL), segments & 1)) { ok = false; break; }
+            tc_fence_after();
+          }
+          const uint32_t qd = q_desc + e * (kTileBytes >> 4), kd = k_desc + ns * (kTileBytes >> 4);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t step = ((ks >> 2) * kBoxBytes + (ks & 3) * 32) / 16;
+            mma_ss(s_at, desc(qd + step), desc(kd + step), idesc_qk, ks > 0, elected);
+          }
+          tc_commit(bar(S_FULL + e), elected);
+          if (e == nne - 1) {
+            tc_commit(bar(K_EMPTY + ns), elected);
+            if (nj + 1 == nj1) tc_commit(bar(Q_EMPTY), elected);
           }
         }
       }
-      for (int e = 0; e < ne; ++e) ++seg_of[e];
-      col = u.first + j1;
-      if (col < end) next_unit(u);
+      // a round on
+      j = nj;
+      ne = on ? nne : 0;
+      limit = nlimit;
+      first = nfirst;
+      nfirst = false;
+      if (on && ++nj == nj1) {
+        on = next_segment(u, nj1);
+        if (on) {
+          nfirst = true;
+          ++segments;
+          nj = 0;
+          nj1 = tiles_to(u);
+          nne = both(u) ? 2 : 1;
+          nlimit = first_limit(u, 0);
+        }
+      }
     }
   } else if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
-    // ---- guards: two keys' values a thread, tiles at the diagonal and the end only ----
-    int guarded = 0;
-    Unit u = begin < end ? unit_at(begin) : Unit{};
-    for (int col = begin; col < end && ok; ++segments) {
+    // ---- guards: a key's values a thread, tiles at the diagonal and the end only ----
+    for (int col = begin; on && ok; ++segments) {
       const int j1 = tiles_to(u), limit = first_limit(u, 0);
       for (int j = tiles_from(u, col); j < j1 && ok; ++j, ++fill) {
-        if (!cut_tile(j, limit)) continue;
-        // (not by V_FULL alone: two tiles further on its phase would look the same as two tiles before)
         const int s = fill % kStages;
-        if (!mbar_wait_bounded(bar(V_GO), guarded++ & 1) || !mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
+        if (!mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
+        if (!cut_tile(j, limit)) {
+          if (lane == 0) mbar_arrive(bar(V_EMPTY + s));
+          continue;
+        }
         bool any = false;
 #pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          const int r = ((warp - 2) * 2 + i) * 32 + lane;
+        for (int r = max(limit + 1 - j * kKeys, 0) + (warp - 2) * 32 + lane; r < kKeys; r += 64) {   // (keys up to `limit` all rows see)
           const bool behind = j * kKeys + r >= u.len;
 #pragma unroll 1
-          for (int c = 0; c < kHalves * 8; ++c) {
-            const uint32_t at = v_smem + s * kTileBytes + (c >> 3) * kBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-            bool write = behind;
+          for (int c0 = 0; c0 < kHalves * 8; c0 += 4) {
+            uint32_t w[4][4], at[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              if (behind) w[x] = 0;
-              if ((w[x] & 0x7f80u) == 0x7f80u) { w[x] &= 0xffff0000u; write = any = true; }
-              if ((w[x] & 0x7f800000u) == 0x7f800000u) { w[x] &= 0xffffu; write = any = true; }
+            for (int c = 0; c < 4; ++c) {
+              at[c] = v_smem + s * kTileBytes + (c0 >> 3) * kBoxBytes + r * 128 + ((((c0 & 7) + c) ^ (r & 7)) << 4);
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3]) : "r"(at[c]) : "memory");
             }
-            if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              bool write = behind;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                if (behind) w[c][x] = 0;
+                if ((w[c][x] & 0x7f80u) == 0x7f80u) { w[c][x] &= 0xffff0000u; write = any = true; }
+                if ((w[c][x] & 0x7f800000u) == 0x7f800000u) { w[c][x] &= 0xffffu; write = any = true; }
+              }
+              if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at[c]), "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3]) : "memory");
+            }
           }
         }
         if (any) odd[segments % kMarks] = 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(V_OK));
+        if (lane == 0) {
+          mbar_arrive(bar(V_OK + s));
+          mbar_arrive(bar(V_EMPTY + s));
+        }
       }
-      col = u.first + j1;
-      if (col < end) next_unit(u);
+      on = next_segment(u, j1);
+      col = u.first;
     }
   } else if (warp < 4 + kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
@@ -367,8 +399,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     constexpr float kLazy = 8.f;                   // log2 of how far the running maximum may outgrow m_ref
     const int token = r / p.R;                     // of the tile
     int g = 0, mine = 0;                           // tiles and segments of this group so far
-    Unit u = begin < end ? unit_at(begin) : Unit{};
-    for (int col = begin; col < end && ok; ++segments) {
+    for (int col = begin; on && ok; ++segments) {
       const int j0 = tiles_from(u, col), j1 = tiles_to(u);
       if (e == 0 || both(u)) {
         const int limit0 = first_limit(u, e), limit = token < cp.tile_tokens ? limit0 + token : -1;   // last key this row may see
@@ -380,7 +411,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, x[c]);
           tc_wait_ld();
-          if (cut_tile(j, limit0)) {
+          if (__builtin_expect(cut_tile(j, limit0), 0)) {
             const int left = min(limit, u.len - 1) - j * kKeys;    // last key of the tile that this row sees
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -402,7 +433,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             if (j > j0) {
               if (!mbar_wait_bounded(bar(O_FULL + e), (g - 1) & 1)) { ok = false; break; }
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 uint32_t y[32];
                 tmem_ld32(to + c * 32, y);
@@ -463,8 +494,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (lane == 0) mbar_arrive(bar(L_FULL + e));
         ++mine;
       }
-      col = u.first + j1;
-      if (col < end) next_unit(u);
+      on = next_segment(u, j1);
+      col = u.first;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOut));
@@ -472,22 +503,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
     int g[2] = {0, 0}, mine[2] = {0, 0};
-    Unit u = begin < end ? unit_at(begin) : Unit{};
     if (r == 0) {      // what the merge has to know of the unit that this run begins in the middle of
       Cut cut = {};
-      if (begin < end && u.first < begin) {
-        cut.first = fd_cta_of(u.first, total, parts);
+      if (begin < end && u.first + kUnitCost < begin) {
+        cut.first = fd_cta_of(u.first + kUnitCost, total, parts);
         if (cut.first == part - 1) {
           cut.b = u.b;
           cut.h = u.h;
           cut.m = u.m;
-          cut.last = fd_cta_of(u.first + u.tiles - 1, total, parts);
+          cut.last = fd_cta_of(u.first + kUnitCost + u.tiles - 1, total, parts);
           cut.parts = cut.last - cut.first + 1;
         }
       }
       cp.cuts[part] = cut;
     }
-    for (int col = begin; col < end && ok; ++segments) {
+    for (int col = begin; on && ok; ++segments) {
       const int j0 = tiles_from(u, col), j1 = tiles_to(u), ne = both(u) ? 2 : 1;
       const bool whole = j0 == 0 && j1 == u.tiles;
       const long long row0 = paged_row0(p, u.b, a.o_sb, a.o_st);
@@ -499,70 +529,93 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         tc_fence_after();
         const int t0 = u.m * block + e * cp.tile_tokens, tokens = min(cp.tile_tokens, u.n - t0);   // tokens of the tile
         const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kMarks) != 0;
-        uint8_t* stage = stage_all + e * (kRows * kSPitch);
         const float inv = lm.x == 0.f ? 0.f : 1.f / lm.x;
         float* rec = part_of<D>(p, part, j0 == 0);
         const uint32_t to = t_o[e] + lane_addr;
+        if (taken) {
+          // values that the guards took out, for the rows that see them: from the cache, key by key, into O_e (a call with such values is lost anyway)
+          const int upto = r < tokens * p.R ? min(min(first_limit(u, e) + r / p.R, u.len - 1), j1 * kKeys - 1) : -1;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t y[32];
-          tmem_ld32(to + c * 32, y);
-          tc_wait_ld();
-          if (taken) {
-            // values that the guards took out, for the rows that see them: from the cache, key by key (a call with such values is lost anyway)
-            const int limit = min(first_limit(u, e) + r / p.R, u.len - 1), from = max(j0 * kKeys, (first_limit(u, 0) + 1) / kKeys * kKeys);
-            const int upto = min(limit, j1 * kKeys - 1);
-            if (r < tokens * p.R)
+          for (int c = 0; c < D; c += 16) {
+            uint32_t y[16];
+            tmem_ld16(to + c, y);
+            tc_wait_ld();
 #pragma unroll 1
-              for (int key = max(from, 0); key <= upto; ++key) {
-                const int page = __ldg(a.page_table + u.b * a.table_st + key / a.page_size);
-                if (page < 0 || page >= a.pages) continue;
-                const uint16_t* v = static_cast<const uint16_t*>(a.cache_v) + page * a.cache_sp + key % a.page_size * a.cache_st + u.h * D + c * 32;
+            for (int key = max(max(j0 * kKeys, first_limit(u, 0) + 1), 0); key <= upto; ++key) {
+              const int page = __ldg(a.page_table + u.b * a.table_st + key / a.page_size);
+              if (page < 0 || page >= a.pages) continue;
+              const uint16_t* v = static_cast<const uint16_t*>(a.cache_v) + page * a.cache_sp + key % a.page_size * a.cache_st + u.h * D + c;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  uint16_t w;
-                  asm volatile("ld.global.u16 %0, [%1];" : "=h"(w) : "l"(v + i));    // (one at a time: registers are few here)
-                  if ((w & 0x7f80) == 0x7f80) y[i] = __float_as_uint(__uint_as_float(y[i]) + __uint_as_float((uint32_t)w << 16));
-                }
+              for (int i = 0; i < 16; ++i) {
+                const uint32_t w = __ldg(v + i);
+                if ((w & 0x7f80u) == 0x7f80u) y[i] = __float_as_uint(__uint_as_float(y[i]) + __uint_as_float(w << 16));
               }
-          }
-          if (whole) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) w[i >> 1] = pack_bf16x2(__uint_as_float(y[i]) * inv, __uint_as_float(y[i + 1]) * inv);
-            uint4* dst = reinterpret_cast<uint4*>(stage + r * kSPitch);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-            asm volatile("bar.sync 2, 128;" ::: "memory");   // the output warpgroup
-#pragma unroll
-            for (int id = r; id < kRows * 4; id += 128) {
-              const int row = id >> 2, ch = id & 3, t = row / p.R;
-              if (t < tokens)
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row0 + (t0 + t) * a.o_st + (long long)(u.h * p.R + row - t * p.R) * a.o_sh + c * 32 + ch * 8) =
-                    *reinterpret_cast<const uint4*>(stage + row * kSPitch + ch * 16);
             }
-            asm volatile("bar.sync 2, 128;" ::: "memory");   // the rows may be written again
-          } else {
+            __syncwarp();
+            tmem_st16(to + c, y);
+            tc_wait_st();
+          }
+        }
+        auto read = [&]() {                                   // O_e and the row's sums are in registers: they may take the next segment's
+          if (e == ne - 1) {
+            asm volatile("bar.sync 2, 128;" ::: "memory");    // (all have read the mark)
+            if (r == 0) odd[segments % kMarks] = 0;
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(O_READ + e));
+        };
+        if (whole) {
+          // 64 columns at a time through the warp's own staging rows: a thread holds one row, a store is to touch few
+          uint8_t* stage = stage_all + q4 * (2 * kRows * kSPitch / 4);
+          constexpr int kPitch = 128 + 16;
+          static_assert(32 * kPitch <= 2 * kRows * kSPitch / 4, "staging rows of a warp");
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 + (long long)(u.h * p.R) * a.o_sh + (lane & 7) * 8;
+#pragma unroll 1
+          for (int h = 0; h < kHalves; ++h) {
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              uint32_t y[32];
+              tmem_ld32(to + h * 64 + c * 32, y);
+              tc_wait_ld();
+              uint4* dst = reinterpret_cast<uint4*>(stage + lane * kPitch + c * 64);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(y[8 * q + 2 * i]) * inv, __uint_as_float(y[8 * q + 2 * i + 1]) * inv);
+                dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+            if (h == kHalves - 1) read();
+            __syncwarp();
+#pragma unroll 2
+            for (int i = 0; i < 8; ++i) {
+              const int row = i * 4 + (lane >> 3), t = (q4 * 32 + row) / p.R;
+              if (t < tokens)
+                *reinterpret_cast<uint4*>(out + (t0 + t) * a.o_st + (q4 * 32 + row - t * p.R) * a.o_sh + h * 64) =
+                    *reinterpret_cast<const uint4*>(stage + row * kPitch + (lane & 7) * 16);
+            }
+            __syncwarp();
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t y[32];
+            tmem_ld32(to + c * 32, y);
+            tc_wait_ld();
+            if (c == D / 32 - 1) read();
 #pragma unroll
             for (int q = 0; q < 8; ++q)
               *reinterpret_cast<uint4*>(rec + ((long long)(c * 8 + q) * (2 * kRows) + e * kRows + r) * 4) = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
           }
-        }
-        if (!whole) {
           rec[2 * kRows * D + e * kRows + r] = lm.y;
           rec[2 * kRows * (D + 1) + e * kRows + r] = lm.x;
         }
-        if (e == ne - 1) {
-          asm volatile("bar.sync 2, 128;" ::: "memory");     // (all have read the mark)
-          if (r == 0) odd[segments % kMarks] = 0;
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(O_READ + e));
         ++mine[e];
       }
-      col = u.first + j1;
-      if (col < end) next_unit(u);
+      on = next_segment(u, j1);
+      col = u.first;
     }
   }
   if (!ok && lane == 0 && a.status) atomicExch(a.status, (int)L3CI_ERR_DEVICE_WAIT);
@@ -647,14 +700,14 @@ __global__ void __launch_bounds__(kMergeThreads) paged_chunk_merge_kernel(const 
 // ---- host ----
 size_t chunk_smem(int D, int B) {
   const size_t tile = (size_t)(D / 64) * 128 * 128;
-  return 1024 + 6 * tile + 2 * kRows * 80 + 23 * 8 + (kMarks + 16) * 4 + 4 * kRows * 4 + (size_t)(B + 1) * 4;
+  return 1024 + 6 * tile + 2 * kRows * 80 + 23 * 8 + (kMarks + 16) * 4 + 4 * kRows * 4 + 16 * sizeof(Unit) + (size_t)(B + 1) * 4;
 }
 
 int chunk_parts(const PagedParams& p) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
   // (columns at most: every token's own unit of all the keys that the table can hold)
   const long long rows = p.a.starts ? p.a.rows : (long long)p.a.B * p.a.T, block = 2 * (kRows / p.R);
-  const long long columns = (rows / block + p.a.B) * p.a.Hkv * (((long long)p.cap + kKeys - 1) / kKeys + 1);
+  const long long columns = (rows / block + p.a.B) * p.a.Hkv * (((long long)p.cap + kKeys - 1) / kKeys + 1 + kUnitCost);
   return (int)(columns < sms ? columns : sms);
 }
 
