@@ -12,38 +12,62 @@
 namespace l3ci {
 namespace {
 
-// z[r, j] = scales[i] x[r] . a[i, j], i = index[r]; 0 without an adapter.  A warp per (r, j).
-__global__ void __launch_bounds__(128) adapter_shrink_kernel(const l3ci_adapter_linear_args p, float* z) {
+// z[r, j] = scales[i] x[r] . a[i, j], i = index[r]; 0 without an adapter.  A CTA per row and kDots ranks, whose warps share the columns of K: a row of
+// x is read once for kDots rows of a, and a warp has all of its loads under way at once (a warp per r and j took 6.2 us for 64 rows of 8192
+// columns and rank 32, and slowed the product's weights, which stream meanwhile, by as much).
+constexpr int kDots = 4, kDotWarps = 4;
+
+__global__ void __launch_bounds__(32 * kDotWarps) adapter_shrink_kernel(const l3ci_adapter_linear_args p, float* z) {
+  __shared__ float parts[kDotWarps][kDots];
   pdl_wait();                // (before the next kernel may start: it reads x and w at once)
   pdl_launch_dependents();
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long long r = item / p.rank;
-  if (r >= p.rows) return;
-  const int j = (int)(item % p.rank), i = p.index[r];
-  float s = 0.f;
-  if (i >= 0 && i < p.adapters) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x, j0 = blockIdx.y * kDots, i = __ldg(p.index + r);
+  const bool has = i >= 0 && i < p.adapters;
+  float s[kDots] = {};
+  if (has) {
     const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + r * p.x_st;
-    const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + ((long long)i * p.rank + j) * p.K;
-    for (int k = lane * 8; k < p.K; k += 256) {
-      float u[8], v[8];
-      unpack8(*reinterpret_cast<const uint4*>(x + k), u);
-      unpack8(*reinterpret_cast<const uint4*>(a + k), v);
+    const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + ((long long)i * p.rank + j0) * p.K;
+#pragma unroll 4
+    for (int k = (warp * 32 + lane) * 8; k < p.K; k += kDotWarps * 256) {
+      const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + k));
+      uint4 av[kDots];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(u[e], v[e], s);
+      for (int j = 0; j < kDots; ++j) av[j] = __ldg(reinterpret_cast<const uint4*>(a + (long long)j * p.K + k));
+      float u[8], v[8];
+      unpack8(xv, u);
+#pragma unroll
+      for (int j = 0; j < kDots; ++j) {
+        unpack8(av[j], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j] = fmaf(u[e], v[e], s[j]);
+      }
     }
-    s = group_sum<32>(s) * (p.scales ? p.scales[i] : 1.f);
   }
-  if (lane == 0) z[item] = s;
+#pragma unroll
+  for (int j = 0; j < kDots; ++j) {
+    s[j] = group_sum<32>(s[j]);
+    if (lane == 0) parts[warp][j] = s[j];
+  }
+  __syncthreads();
+  if (threadIdx.x < kDots) {
+    float y = 0.f;
+    for (int w = 0; w < kDotWarps; ++w) y += parts[w][threadIdx.x];
+    z[(long long)r * p.rank + j0 + threadIdx.x] = has ? y * (p.scales ? __ldg(p.scales + i) : 1.f) : 0.f;
+  }
 }
 
 // The same of many rows, on the tensor cores: 32 rows of x a CTA, warps share the columns of K and add up at the end.  A dot product does not
 // ask in which order its terms come: a lane takes 8 neighbouring columns, 16 bytes, of a row of x and of a row of a, which are the operands of two
 // products.  Of every adapter among the 32 rows all rows' products are computed and its own rows' kept.
 // CTAs behind these list the adapters among every 256 rows (linear_many.h).
-constexpr int kShrinkRows = 32, kShrinkWarps = 8, kShrinkRanks = 32;   // ranks at a time: four products wide
+constexpr int kShrinkRows = 32, kShrinkWarps = 8;
 
-__global__ void __launch_bounds__(32 * kShrinkWarps) adapter_shrink_many_kernel(const l3ci_adapter_linear_args p, float* z, int* lists, int blocks) {
+// NT: products of 8 ranks side by side.  (Two CTAs an SM: 6001 rows are then one wave.  16 warps at 128 registers, one CTA an SM, took 17.5 us for
+// them at K = 2048, rank 16.)
+template <int NT>
+__global__ void __launch_bounds__(32 * kShrinkWarps, 2) adapter_shrink_many_kernel(const l3ci_adapter_linear_args p, float* z, int* lists, int blocks) {
+  constexpr int kShrinkRanks = 8 * NT;   // ranks at a time
   __shared__ float parts[kShrinkWarps][kShrinkRows][kShrinkRanks + 1];
   __shared__ int ids[kAdapterTile];
   pdl_wait();
@@ -55,9 +79,9 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) adapter_shrink_many_kernel(
   };
   if ((int)blockIdx.x >= blocks) {       // ---- a list ----
     const int t = threadIdx.x, tile = blockIdx.x - blocks;
-    ids[t] = id_of((long long)tile * kAdapterTile + t);
+    if (t < kAdapterTile) ids[t] = id_of((long long)tile * kAdapterTile + t);
     __syncthreads();
-    bool first = ids[t] >= 0;            // the first row of its adapter
+    bool first = t < kAdapterTile && ids[t] >= 0;            // the first row of its adapter
     for (int i = 0; i < t && first; ++i) first = ids[i] != ids[t];
     int* counts = reinterpret_cast<int*>(parts);
     const unsigned mask = __ballot_sync(kFullMask, first);
@@ -69,8 +93,16 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) adapter_shrink_many_kernel(
       all += counts[w];
     }
     int* list = lists + (long long)tile * kAdapterList;
-    if (first) list[1 + at] = ids[t];
     if (t == 0) list[0] = all;
+    if (first) {
+      int* entry = list + kAdapterHead + at * kAdapterEntry;
+      entry[0] = ids[t];
+      for (int w = 0; w < kAdapterTile / 32; ++w) {
+        unsigned others = 0;
+        for (int i = 0; i < 32; ++i) others |= (unsigned)(ids[w * 32 + i] != ids[t]) << i;
+        entry[4 + w] = (int)others;
+      }
+    }
     return;
   }
   const long long row0 = (long long)blockIdx.x * kShrinkRows;
@@ -92,19 +124,20 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) adapter_shrink_many_kernel(
     for (int j0 = 0; j0 < p.rank; j0 += kShrinkRanks) {
       const int tiles = min(p.rank - j0, kShrinkRanks) / 8;
       const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + ((long long)id * p.rank + j0 + gid) * p.K + tig * 8;
-      float acc[2][4][4] = {};
-#pragma unroll 2
+      float acc[2][NT][4] = {};
+      constexpr int kAhead = NT > 2 ? 2 : 4;
+#pragma unroll kAhead
       for (int k = warp * 32; k < p.K; k += kShrinkWarps * 32) {
         const bool in = k + tig * 8 < p.K;                 // (K is a multiple of 8)
-        uint4 xv[4], av[4];
+        uint4 xv[4], av[NT];
 #pragma unroll
         for (int i = 0; i < 4; ++i) xv[i] = in ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) av[n] = in && n < tiles ? __ldg(reinterpret_cast<const uint4*>(a + (long long)n * 8 * p.K + k)) : make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < NT; ++n) av[n] = in && n < tiles ? __ldg(reinterpret_cast<const uint4*>(a + (long long)n * 8 * p.K + k)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
+          for (int n = 0; n < NT; ++n) {
             mma_bf16(acc[m][n], xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y, av[n].x, av[n].y);
             mma_bf16(acc[m][n], xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w, av[n].z, av[n].w);
           }
@@ -112,7 +145,7 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) adapter_shrink_many_kernel(
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) parts[warp][m * 16 + gid + (e >> 1) * 8][n * 8 + 2 * tig + (e & 1)] = acc[m][n][e];
       __syncthreads();
@@ -150,11 +183,24 @@ int check(const l3ci_adapter_linear_args* a) {
 namespace l3ci {
 namespace {
 
+// Whether the call goes to the product of few rows (64 at a time, weights on the wide side of the tensor cores, low-rank parts in multiply-adds) or to
+// that of many (tiles of 256 x 256 over pairs of SMs).  Estimates in us, fits to both sides on a B200, e.g. rank 16, 2 adapters, few and many: rows 128,
+// 2048 -> 8192 19 and 27, 512 62 and 27; 8192 -> 2048 rows 512 35 and 72; 4096 -> 4096 rows 256 21 and 42, 512 39 and 42; rank 64, 8
+// adapters: 2048 -> 8192 rows 128 41 and 55, 256 105 and 42.
+bool few_rows(const l3ci_adapter_linear_args* a) {
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  const long long groups = (a->rows + L3CI_LINEAR_MAX_ROWS - 1) / L3CI_LINEAR_MAX_ROWS;
+  const long long tiles = (a->rows + kAdapterTile - 1) / kAdapterTile * ((a->N + 255) / 256), pairs = sms / 2 > 0 ? sms / 2 : 1;
+  const double few = 9.0 + 7.7e-8 * groups * a->N * a->K + 7e-7 * a->rows * a->N * a->rank;
+  const double many = 11.0 + 0.0076 * a->K * ((tiles + pairs - 1) / pairs);
+  return few <= many;
+}
+
 // Scratch: z, then the lists of many rows.
 size_t z_bytes(const l3ci_adapter_linear_args* a) { return ((size_t)a->rows * a->rank * 4 + 15) / 16 * 16; }
 size_t scratch_of(const l3ci_adapter_linear_args* a) {
   const size_t tiles = ((size_t)a->rows + kAdapterTile - 1) / kAdapterTile;
-  return z_bytes(a) + (a->rows > L3CI_LINEAR_MAX_ROWS ? tiles * kAdapterList * 4 : 0);
+  return z_bytes(a) + (few_rows(a) ? 0 : tiles * kAdapterList * 4);
 }
 
 }  // namespace
@@ -180,12 +226,16 @@ extern "C" int l3ci_adapter_linear(const l3ci_adapter_linear_args* a) {
   l.K = a->K; l.N = a->N; l.groups = 1;
   l.stream = a->stream;
   const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(a->b);
-  if (a->rows <= L3CI_LINEAR_MAX_ROWS) {
-    L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)((a->rows * a->rank + 3) / 4)), dim3(128), 0, stream, *a, z);
+  if (few_rows(a)) {
+    L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)a->rows, (unsigned)(a->rank / kDots)), dim3(32 * kDotWarps), 0, stream, *a, z);
     return adapter_rows_launch(&l, AdapterRows{z, a->index, b, a->rank, a->adapters});
   }
   int* lists = reinterpret_cast<int*>(static_cast<uint8_t*>(a->scratch) + z_bytes(a));
   const long long blocks = (a->rows + kShrinkRows - 1) / kShrinkRows, tiles = (a->rows + kAdapterTile - 1) / kAdapterTile;
-  L3CI_LAUNCH("adapter_shrink_many_kernel", adapter_shrink_many_kernel, dim3((unsigned)(blocks + tiles)), dim3(32 * kShrinkWarps), 0, stream, *a, z, lists, (int)blocks);
-  return adapter_many_launch(&l, AdapterMany{z, a->index, b, lists, a->rank, a->adapters});
+  auto shrink = [&](auto kernel) -> int {
+    L3CI_LAUNCH("adapter_shrink_many_kernel", kernel, dim3((unsigned)(blocks + tiles)), dim3(32 * kShrinkWarps), 0, stream, *a, z, lists, (int)blocks);
+    return L3CI_OK;
+  };
+  if (int st = a->rank <= 8 ? shrink(adapter_shrink_many_kernel<1>) : a->rank <= 16 ? shrink(adapter_shrink_many_kernel<2>) : shrink(adapter_shrink_many_kernel<4>)) return st;
+  return adapter_many_launch(&l, AdapterMany{z, b, lists, a->rank, a->adapters});
 }

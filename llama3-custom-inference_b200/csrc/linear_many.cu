@@ -38,7 +38,6 @@ constexpr int kPieceBytes = kHalf * kPieceCols * 2;
 constexpr int kThreads = 32 * (4 + kOutWarps);   // producer, MMA issue, allocation, none; outputs
 constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kBox + kOutWarps / 4 * kPieceBytes;
 constexpr size_t kAdaptSmem = kSmem + 2 * kBox;   // with the two boxes of z
-constexpr int kMarks = 4;                  // tiles with adapters whose marks are kept: the filling warps are at most three of them ahead of the output warps
 
 __device__ int g_wait_status = 0;
 
@@ -120,16 +119,19 @@ __device__ __forceinline__ float silu_mul(float z, float u) {
   return bf16_of(__fdividef(z * 0.0625f, fmaf(__expf(-z), 0.0625f, 0.0625f))) * bf16_of(u);
 }
 
-__device__ __forceinline__ bool no_numbers(const uint4& v) {   // a bf16 that is NaN or infinite among eight
-  auto any = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
-  return any(v.x) || any(v.y) || any(v.z) || any(v.w);
+// The same for some of the 256 rows: the accumulators of the others (bits set in `off`) are not touched.
+__device__ __forceinline__ void pair_mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&off)[8], uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.eq.b32 p, 0, 0;\n\tsetp.ne.b32 q, %12, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7]), "r"(elected)
+      : "memory");
 }
 
-// ADAPT: low-rank parts beside the product (l3ci_adapter_linear), as further columns: behind a tile's K columns come, for every adapter among its
-// 256 rows, the adapter's b as w and its rows' z as x, zeros in the rows of others, so that the parts land in the same accumulator and
-// are rounded once with it.  z is fp32: it goes in as two bf16 that add up to 2^-17 of it.  The boxes of z are written by two warps of each CTA
-// (while the K columns run).  0 times what is no number is none: an adapter whose b holds such values in the tile's columns is left out,
-// and its rows' parts are added by the output warps in multiply-adds.
+// ADAPT: low-rank parts beside the product (l3ci_adapter_linear), as further columns: behind a tile's K columns come z of its rows as x and, for every
+// adapter among them, the adapter's b as w, in products that leave the rows of others alone; the parts land in the same accumulator and are
+// rounded once with it, and no row meets another's adapter (zeros in the place of other rows' z would, where a b is no number).  z is fp32: it goes in
+// as two bf16 that add up to 2^-17 of it, written by two warps of each CTA while the K columns run.
 template <int ACT, bool ADAPT>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap bmap,
@@ -140,8 +142,6 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* out_box = smem + kStages * 2 * kBox;
   const uint32_t z_box = smem_u32(smem + kSmem - 1024);            // ADAPT: the upper halves of z, then what they leave
-  __shared__ uint8_t marks[ADAPT ? kMarks : 1][kHalf];             // ADAPT: rows whose parts are the output warps'
-  __shared__ int left_out;                                         // ADAPT: the filled boxes are not to be multiplied
   __shared__ __align__(8) uint64_t bars[2 * kStages + 6];
   __shared__ uint32_t tmem_slot;
   const uint32_t ring = smem_u32(smem), full0 = smem_u32(bars), empty0 = full0 + kStages * 8, done0 = empty0 + kStages * 8, read0 = done0 + 16,
@@ -176,7 +176,7 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   pdl_launch_dependents();
   pdl_wait();
   const int chunks = ADAPT ? (p.low.rank + kDeep - 1) / kDeep : 0;             // columns of z of one adapter, 64 at a time
-  auto list_of = [&](long long tile) { return p.low.lists + tile % p.m_tiles * kAdapterList; };   // number, then the adapters among a tile's rows
+  auto list_of = [&](long long tile) { return p.low.lists + tile % p.m_tiles * kAdapterList; };
   bool ok = true;
   int asked = 0;
 
@@ -199,11 +199,15 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         }
         if constexpr (ADAPT) {
           const int* list = list_of(tile);
-          for (int i = 0; i < list[0] * chunks && ok; ++i) {
+          const int count = list[0];
+          int id = count > 0 ? list[kAdapterHead] : 0;
+          for (int i = 0; i < count * chunks && ok; ++i) {
+            const int next = list[kAdapterHead + (i + 1) % count * kAdapterEntry];     // (asked for a round ahead)
             if (!mbar_wait_bounded_one(empty0 + s * 8, parity)) { ok = false; break; }
             ++asked;
             if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * kBox);
-            pair_load(ring + s * 2 * kBox + kBox, &bmap, first_cta(full0 + s * 8), i % chunks * kDeep, col, list[1 + i / chunks]);
+            pair_load(ring + s * 2 * kBox + kBox, &bmap, first_cta(full0 + s * 8), i / count * kDeep, col, id);
+            id = next;
             if (++s == kStages) { s = 0; parity ^= 1; }
           }
         }
@@ -236,78 +240,65 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         if (++s == kStages) { s = 0; parity ^= 1; }
       }
       if constexpr (ADAPT) {
-        const int count = ok ? list_of(tile)[0] * chunks : 0;
-        for (int i = 0; i < count; ++i, ++filled) {
-          if (!mbar_wait_bounded(full0 + s * 8, parity) || !mbar_wait_bounded(z_full, filled & 1)) { ok = false; break; }
+        const int* list = list_of(tile);
+        const int count = ok ? list[0] : 0;
+        uint32_t off[8];
+        auto rows_off = [&](int i) {               // the rows of the others
+          const uint4* m = reinterpret_cast<const uint4*>(list + kAdapterHead + i % count * kAdapterEntry + 4);
+          const uint4 x = __ldg(m), y = __ldg(m + 1);
+          off[0] = x.x; off[1] = x.y; off[2] = x.z; off[3] = x.w; off[4] = y.x; off[5] = y.y; off[6] = y.z; off[7] = y.w;
+        };
+        if (count > 0) rows_off(0);
+        for (int i = 0; i < count * chunks; ++i) {
+          if (!mbar_wait_bounded(full0 + s * 8, parity) || (i % count == 0 && !mbar_wait_bounded(z_full, filled++ & 1))) { ok = false; break; }
           tc_fence_after();
-          if (!*reinterpret_cast<volatile int*>(&left_out)) {
-            const uint64_t zd = smem_desc(z_box, 16, 1024), ld = smem_desc(z_box + kBox, 16, 1024), bd = smem_desc(ring + s * 2 * kBox + kBox, 16, 1024);
-            const int steps = (min(p.low.rank - i % chunks * kDeep, kDeep) + 15) / 16;
-            for (int k = 0; k < steps; ++k) pair_mma(tmem + acc * kCols, zd + k * 2, bd + k * 2, idesc, 1u, elected);
-            for (int k = 0; k < steps; ++k) pair_mma(tmem + acc * kCols, ld + k * 2, bd + k * 2, idesc, 1u, elected);
+          const uint64_t zd = smem_desc(z_box, 16, 1024), ld = smem_desc(z_box + kBox, 16, 1024), bd = smem_desc(ring + s * 2 * kBox + kBox, 16, 1024);
+          const int steps = (min(p.low.rank - i / count * kDeep, kDeep) + 15) / 16;
+          for (int k = 0; k < steps; ++k) {
+            pair_mma_rows(tmem + acc * kCols, zd + k * 2, bd + k * 2, idesc, off, elected);
+            pair_mma_rows(tmem + acc * kCols, ld + k * 2, bd + k * 2, idesc, off, elected);
           }
           pair_commit(empty0 + s * 8, elected);
-          pair_commit(z_empty, elected);
+          if (i % count == count - 1) pair_commit(z_empty, elected);
           if (++s == kStages) { s = 0; parity ^= 1; }
+          if (i + 1 < count * chunks) rows_off(i + 1);
         }
       }
       if (ok) pair_commit(done0 + acc * 8, elected);
     }
   } else if (ADAPT && (warp == 2 || warp == 3)) {
     // ---- ADAPT: boxes of z, two rows a lane ----
-    const AdapterMany& d = p.low;
-    int listed = 0, filled = 0;          // tiles with adapters, boxes
+    int filled = 0;
     for (long long tile = pair; tile < p.tiles && ok; tile += pairs) {
-      const int row0 = (int)(tile % p.m_tiles) * 2 * kHalf + (int)rank * kHalf, col = (int)(tile / p.m_tiles) * kOuts;
-      const int* list = list_of(tile);
-      if (list[0] == 0) continue;
-      uint8_t* mark = marks[listed++ % kMarks];
-      const int r[2] = {(warp - 2) * 64 + lane, (warp - 2) * 64 + 32 + lane};
-      int id[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        id[i] = row0 + r[i] < p.rows ? __ldg(d.index + row0 + r[i]) : -1;
-        mark[r[i]] = 0;
-      }
-      for (int a = 0; a < list[0] && ok; ++a) {
-        const int adapter = list[1 + a];
-        // (the columns of both CTAs, so that both decide alike)
-        const uint4* b = reinterpret_cast<const uint4*>(d.b + ((long long)adapter * p.N + col) * d.rank);
-        const int vecs = min(2 * kHalf, p.N - col) * (d.rank / 8);
-        bool odd = false;
-#pragma unroll 4
-        for (int v = lane; v < vecs; v += 32) odd |= no_numbers(__ldg(b + v));
-        odd = __any_sync(kFullMask, odd);
-        for (int c = 0; c < chunks; ++c, ++filled) {
-          if (filled > 0 && !mbar_wait_bounded(z_empty, (filled - 1) & 1)) { ok = false; break; }
-          const int wide = min(d.rank - c * kDeep, kDeep);
+      if (list_of(tile)[0] == 0) continue;
+      const int row0 = (int)(tile % p.m_tiles) * 2 * kHalf + (int)rank * kHalf;
+      for (int c = 0; c < chunks; ++c, ++filled) {
+        if (filled > 0 && !mbar_wait_bounded(z_empty, (filled - 1) & 1)) { ok = false; break; }
+        const int wide = min(p.low.rank - c * kDeep, kDeep);
 #pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            const bool mine = id[i] == adapter && !odd;
-            if (id[i] == adapter && odd) mark[r[i]] = 1;
-            const float4* z = reinterpret_cast<const float4*>(d.z + (long long)(row0 + r[i]) * d.rank + c * kDeep);
-#pragma unroll 2
-            for (int v = 0; v < kDeep / 8; ++v) {
-              uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-              if (mine && v * 8 < wide) {
-                const float4 f0 = __ldg(z + 2 * v), f1 = __ldg(z + 2 * v + 1);
-                float f[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w}, h[8];
-                hi = pack8(f);
-                unpack8(hi, h);
+        for (int v = 0; v * 8 < (wide + 15) / 16 * 16; ++v) {      // (columns that a product reads; rows without an adapter hold anything)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = fabsf(h[e]) < INFINITY ? f[e] - h[e] : 0.f;   // (what is no number goes in once)
-                lo = pack8(f);
-              }
-              const uint32_t at = z_box + r[i] * 128 + ((v ^ (r[i] & 7)) << 4);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + kBox), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+          for (int i = 0; i < 2; ++i) {
+            const int r = (warp - 2) * 64 + i * 32 + lane;
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            if (row0 + r < p.rows && v * 8 < wide) {
+              const float4* z = reinterpret_cast<const float4*>(p.low.z + (long long)(row0 + r) * p.low.rank + c * kDeep + v * 8);
+              const float4 f0 = __ldg(z), f1 = __ldg(z + 1);
+              float f[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w}, h[8];
+              hi = pack8(f);
+              unpack8(hi, h);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = fabsf(h[e]) < INFINITY ? f[e] - h[e] : 0.f;   // (what is no number goes in once)
+              lo = pack8(f);
             }
+            const uint32_t at = z_box + r * 128 + ((v ^ (r & 7)) << 4);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + kBox), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
           }
-          if (warp == 2 && lane == 0) left_out = odd;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) arrive_cluster(first_cta(z_full));
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_cluster(first_cta(z_full));
       }
     }
     // (the last arrival on z_empty comes from the pair's products: this CTA must not leave ahead of it)
@@ -319,7 +310,7 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     uint8_t* box = out_box + part * kPieceBytes;
     constexpr int kShare = kOuts / (kOutWarps / 4);
     auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory"); };
-    int round = 0, listed = 0;
+    int round = 0;
     for (long long tile = pair; tile < p.tiles && ok; tile += pairs, ++round) {
       const int acc = round & 1;
       const int row = (int)(tile % p.m_tiles) * 2 * kHalf + (int)rank * kHalf, col = (int)(tile / p.m_tiles) * kOuts;
@@ -331,9 +322,6 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       }
       if (!ok) break;
       tc_fence_after();
-      bool marked = false;                     // (the filling warps have written the marks ahead of the boxes that the products waited for)
-      if constexpr (ADAPT)
-        if (list_of(tile)[0] > 0) marked = *const_cast<volatile uint8_t*>(&marks[listed++ % kMarks][r]) != 0;
 #pragma unroll 1
       for (int c0 = part * kShare; c0 < (part + 1) * kShare; c0 += kPieceCols) {
         meet();                                // the box has been read
@@ -354,17 +342,6 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
               else if (GATED) f[i] = gated_activation(f[i], __uint_as_float(z[v * 8 + i]), 0.f, 0.f);
               else if (ACT == L3CI_ACT_TANH) f[i] = tanhf(f[i]);
             }
-            if (marked)                        // (z b of a row whose adapter was left out)
-              for (int i = 0; i < 8; ++i) {
-                const int n = col + c0 + c + v * 8 + i;
-                if (n >= p.N) break;
-                const float* z = p.low.z + (long long)(row + r) * p.low.rank;
-                const __nv_bfloat16* b = p.low.b + ((long long)__ldg(p.low.index + row + r) * p.N + n) * p.low.rank;
-                float y = 0.f;
-                for (int k = 0; k < p.low.rank; ++k) y = fmaf(__ldg(z + k), __bfloat162float(b[k]), y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] += e == i ? y : 0.f;
-              }
             if (ACT == L3CI_ACT_GELU)
 #pragma unroll
               for (int i = 0; i < 8; i += 2) gelu(f[i], f[i + 1]);

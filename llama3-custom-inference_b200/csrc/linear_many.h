@@ -11,12 +11,12 @@ namespace l3ci {
 // The device word where its waits that ran out are recorded (of the current device); null without a device.
 int* linear_many_wait_status();
 
-// Low-rank parts beside a product of many rows, as AdapterRows (linear_rows.h) beside one of few, and for every 256 rows a list of kAdapterList
-// words: the number of adapters among them, then these.
-constexpr int kAdapterTile = 256, kAdapterList = 1 + kAdapterTile;
+// Low-rank parts beside a product of many rows, as AdapterRows (linear_rows.h) beside one of few, and for every 256 rows a list of kAdapterList words, on 16
+// bytes: the number of adapters among them, then, from kAdapterHead on, an entry of kAdapterEntry words for each: its number at 0, and from 4 on a bit
+// for each of the 256 rows that is NOT its own.  z of rows without an adapter may hold anything.
+constexpr int kAdapterTile = 256, kAdapterHead = 4, kAdapterEntry = 12, kAdapterList = kAdapterHead + kAdapterTile * kAdapterEntry;
 struct AdapterMany {
   const float* z;
-  const int32_t* index;
   const __nv_bfloat16* b;
   const int* lists;
   int rank, adapters;

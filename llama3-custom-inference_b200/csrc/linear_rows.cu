@@ -114,7 +114,8 @@ __device__ __forceinline__ bool output_warps_agree(bool ok) {
 // ADAPT: every token's low-rank part z b[i]^T (l3ci_adapter_linear) is added to the sums.  The output warps, which have nothing to do while the
 // tensor cores run, compute it in multiply-adds from z in 32 bits, a token after the other: B of the adapters in use is read beside w, a token
 // meets no other's adapter, and nothing waits for it but the stores.  The kernel ahead (adapter_linear.cu) waits for its own predecessors
-// before it lets this one start: w and x may be read at once, and stream while it computes z.
+// before it lets this one start: w and x may be read at once, and stream while it computes z.  More than 64 tokens are groups of 64 that read the
+// same w, neighbours in the order of the tiles, which meet it in L2.
 template <int NP, int S, int GATE, bool ROPE, bool ADAPT>
 __global__ void __launch_bounds__(kThreads, 2)
 linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ LinParams p) {
@@ -190,25 +191,54 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   float low[kMine];
   // (numbered by the rows of the accumulator that the warp may read)
   const int out_thread = (warp & 3) * 32 + lane, tok0 = out_thread / kOwn;
-  float* zs = reinterpret_cast<float*>(tmem_slot + 4);              // [rows][rank], then the rows' adapters
-  auto low_rank = [&](int n) {
+  // of a tile: its group, its first row of w, the group's rows
+  auto group_of = [&](int tile) { return ADAPT ? tile % a.groups : tile / p.group_tiles; };
+  auto row_of = [&](int tile) { return (ADAPT ? tile / a.groups : tile % p.group_tiles) * kOuts; };
+  auto rows_of = [&](int grp) { return ADAPT ? (int)min((long long)NP, a.rows - (long long)grp * NP) : (int)a.rows; };
+  auto low_rank = [&](int n, int grp, int rows) {
     const AdapterRows& d = p.low;
-    const int* ids = reinterpret_cast<const int*>(zs + (int)a.rows * d.rank);
 #pragma unroll
     for (int i = 0; i < kMine; ++i) low[i] = 0.f;
     if (n >= a.N) return;
-    for (int r = 0; r < d.rank; r += 8) {
+    const int32_t* index = d.index + (long long)grp * NP;
+    const float* z = d.z + (long long)grp * NP * d.rank;       // (by L1: in shared memory it would cost a CTA per SM from rank 40 on)
+    const __nv_bfloat16* b = d.b + (long long)n * d.rank;
+    const long long one = (long long)a.N * d.rank;
+    // (vectors of several tokens under way at once)
+    constexpr int kAhead = kMine < 8 ? kMine : 8;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int t = tok0 + i * S;
-        if (t >= (int)a.rows) break;
-        const int id = ids[t];
-        if (id < 0) continue;
-        float f[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(d.b + ((long long)id * a.N + n) * d.rank + r)), f);
-        const float4 z0 = *reinterpret_cast<const float4*>(zs + t * d.rank + r), z1 = *reinterpret_cast<const float4*>(zs + t * d.rank + r + 4);
-        low[i] = fmaf(z0.x, f[0], fmaf(z0.y, f[1], fmaf(z0.z, f[2], fmaf(z0.w, f[3], low[i]))));
-        low[i] = fmaf(z1.x, f[4], fmaf(z1.y, f[5], fmaf(z1.z, f[6], fmaf(z1.w, f[7], low[i]))));
+    for (int i0 = 0; i0 < kMine; i0 += kAhead) {
+      if (tok0 + i0 * S >= rows) break;
+      int id[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int t = tok0 + (i0 + i) * S;
+        id[i] = t < rows ? __ldg(index + t) : -1;
+        if (id[i] >= d.adapters) id[i] = -1;
+      }
+#pragma unroll 1
+      for (int r = 0; r < d.rank; r += 8) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          // (rows of b lie apart: a load touches a line for every lane, and a neighbour of the same adapter spares it)
+          const bool same = i > 0 && id[i] == id[i > 0 ? i - 1 : 0];
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (id[i] >= 0 && !same) v[i] = __ldg(reinterpret_cast<const uint4*>(b + id[i] * one + r));
+        }
+#pragma unroll
+        for (int i = 1; i < kAhead; ++i)
+          if (id[i] == id[i - 1]) v[i] = v[i - 1];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const float4* zt = reinterpret_cast<const float4*>(z + (long long)min(tok0 + (i0 + i) * S, rows - 1) * d.rank + r);
+          const float4 z0 = __ldg(zt), z1 = __ldg(zt + 1);
+          float f[8];
+          unpack8(v[i], f);
+          float& y = low[i0 + i];
+          y = fmaf(z0.x, f[0], fmaf(z0.y, f[1], fmaf(z0.z, f[2], fmaf(z0.w, f[3], y))));
+          y = fmaf(z1.x, f[4], fmaf(z1.y, f[5], fmaf(z1.z, f[6], fmaf(z1.w, f[7], y))));
+        }
       }
     }
   };
@@ -221,7 +251,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy_x));
       // (one thread's instructions are all that a stage waits for: counters, no divisions, on the way to a copy)
       struct At { int tile, grp, row, k; };
-      auto at_tile = [&](int tile) { return At{tile, tile / p.group_tiles, tile % p.group_tiles * kOuts, 0}; };
+      auto at_tile = [&](int tile) { return At{tile, group_of(tile), row_of(tile), 0}; };
       auto advance = [&](At& t) {
         if (++t.k == steps) t = at_tile(t.tile + stride);
       };
@@ -229,11 +259,11 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         const uint32_t dst = ring + s * Sh::kStageBytes, bar = full0 + s * 8;
         ++asked;
         mbar_expect_tx(bar, Sh::kStageBytes);
-        tma_load_4d(dst, &wmap, bar, (k0 + t.k) * kDeep, t.row, 0, t.grp, policy_w);
+        tma_load_4d(dst, &wmap, bar, (k0 + t.k) * kDeep, t.row, 0, ADAPT ? 0 : t.grp, policy_w);
         if (GATED) tma_load_4d(dst + kWBytes / 2, &wmap, bar, (k0 + t.k) * kDeep, t.row, 1, t.grp, policy_w);
       };
       auto load_x = [&](int s, const At& t) {
-        tma_load_4d(ring + s * Sh::kStageBytes + kWBytes, &xmap, full0 + s * 8, (k0 + t.k) * kDeep, 0, 0, t.grp, policy_x);
+        tma_load_4d(ring + s * Sh::kStageBytes + kWBytes, &xmap, full0 + s * 8, (k0 + t.k) * kDeep, ADAPT ? t.grp * NP : 0, 0, ADAPT ? 0 : t.grp, policy_x);
       };
       if (!ADAPT && !a.early) pdl_wait();
       At w = at_tile(first), x = w;
@@ -277,30 +307,22 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     // ---- output: a thread owns row r of the tile ----
     pdl_wait();
     if constexpr (ROPE) pair = pair_at((int)threadIdx.x - 64);
-    if constexpr (ADAPT) {
-      const int count = (int)a.rows * p.low.rank;
-      int* ids = reinterpret_cast<int*>(zs + count);
-      for (int i = out_thread; i < count / 4; i += 128) reinterpret_cast<float4*>(zs)[i] = __ldcg(reinterpret_cast<const float4*>(p.low.z) + i);
-      for (int i = out_thread; i < (int)a.rows; i += 128) {
-        const int id = __ldg(p.low.index + i);
-        ids[i] = id < p.low.adapters ? id : -1;
-      }
-      output_warps_meet();
-      if constexpr (S > 1) low_rank(first * kOuts + rank * kOwn + out_thread % kOwn);
+    if constexpr (ADAPT && S > 1) {
+      const int grp = group_of(first);
+      low_rank(row_of(first) + rank * kOwn + out_thread % kOwn, grp, rows_of(grp));
     }
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
-    const int rows = (int)a.rows;
     int round = 0;
     for (int tile = first; tile < p.tiles; tile += stride, ++round) {
-      const int acc = round & 1;
-      if constexpr (ADAPT && S == 1) low_rank(tile * kOuts + out_thread);
+      const int acc = round & 1, rows = rows_of(group_of(tile));
+      if constexpr (ADAPT && S == 1) low_rank(row_of(tile) + out_thread, group_of(tile), rows);
       ok = mbar_wait_bounded(done0 + acc * 8, (round >> 1) & 1);
       if (GATED && S == 1) ok = output_warps_agree(ok);
       if (!ok) break;
       tc_fence_after();
       if constexpr (S == 1) {
-        const int grp = tile / p.group_tiles, n = tile % p.group_tiles * kOuts + (GATED ? r & 63 : r);
+        const int grp = group_of(tile), n = row_of(tile) + (GATED ? r & 63 : r);
 #pragma unroll
         for (int c = 0; c < NP; c += 16) {
           if (c >= rows) break;
@@ -340,7 +362,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     if constexpr (Sh::kInRing) cluster_arrive();
     cluster_wait();                                       // the others' shared memory may be written: they have started, or are done with the ring
     if (warp >= 2 && ok) {
-      const int q4 = warp & 3, r = q4 * 32 + lane, rows = (int)a.rows;
+      const int q4 = warp & 3, r = q4 * 32 + lane, rows = rows_of(group_of(first));
       const int j = GATED ? r & 63 : r;
       // [token][rank][row of the slice]: a warp's stores of one token are neighbours (16-byte stores of four tokens each, which are
       // not, were slower)
@@ -383,16 +405,16 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       }
     }
     if constexpr (ADAPT) {
-      const int j = out_thread % kOwn, n = first * kOuts + rank * kOwn + j;
+      const int j = out_thread % kOwn, n = row_of(first) + rank * kOwn + j, grp = group_of(first), rows = rows_of(grp);
       if (warp >= 2 && n < a.N)
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
           const int t = tok0 + i * S;
-          if (t >= (int)a.rows) break;
+          if (t >= rows) break;
           float y = low[i];
 #pragma unroll
           for (int s = 0; s < S; ++s) y += parts[t * kTile + s * kSlice + j];
-          store_out(a, 0, t, n, y);
+          store_out(a, grp, t, n, y);
         }
     }
     for (int e = threadIdx.x; !ROPE && !ADAPT && e < (int)a.rows * kOwn; e += kThreads) {
@@ -427,27 +449,27 @@ int launch(const l3ci_linear_args* a, float limit, float alpha, cudaStream_t str
   p.alpha = alpha;
   if (rope) p.rope = *rope;
   if (low) p.low = *low;
-  const size_t smem = Sh::kSmem + (low ? (size_t)a->rows * (low->rank + 1) * 4 : 0);
   p.group_tiles = (a->N + kOuts - 1) / kOuts;
   p.tiles = p.group_tiles * a->groups;
   p.steps = (a->K + kDeep - 1) / kDeep;
   const long long one = (long long)a->N * a->K;
   CUtensorMap xmap, wmap;
-  if (int st = make_rows_map(&xmap, a->x, a->K, (int)a->rows, 1, a->groups, a->x_st, 0, a->x_sg, NP)) return st;
-  if (int st = make_rows_map(&wmap, a->w, a->K, a->N, GATED ? 2 : 1, a->groups, a->K, one, one * (GATED ? 2 : 1), kOuts)) return st;
+  const int stacks = ADAPT ? 1 : a->groups;     // of rows of x and w
+  if (int st = make_rows_map(&xmap, a->x, a->K, (int)a->rows, 1, stacks, a->x_st, 0, a->x_sg, NP)) return st;
+  if (int st = make_rows_map(&wmap, a->w, a->K, a->N, GATED ? 2 : 1, stacks, a->K, one, one * (GATED ? 2 : 1), kOuts)) return st;
   auto kernel = linear_rows_kernel<NP, S, GATE, ROPE, ADAPT>;
   static bool configured[64] = {false};
   int dev = 0;
   L3CI_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    L3CI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Sh::kSmem + (ADAPT ? NP * (L3CI_ADAPTER_MAX_RANK + 1) * 4 : 0))));
+    L3CI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::kSmem));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count() > 0 ? sm_count() : 148;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(S > 1 ? p.tiles * S : p.tiles < 2 * sms ? p.tiles : 2 * sms));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = Sh::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -495,7 +517,7 @@ int launch_split(const l3ci_linear_args* a, float limit, float alpha, cudaStream
 
 template <int NP>
 int launch_adapters(const l3ci_linear_args* a, const AdapterRows* low, cudaStream_t stream) {
-  switch (split_for((a->N + kTile - 1) / kTile, a->K)) {
+  switch (split_for((a->N + kTile - 1) / kTile * (long long)a->groups, a->K)) {
     case 1: return launch<NP, 1, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
     case 2: return launch<NP, 2, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
     case 4: return launch<NP, 4, 0, false, true>(a, 0.f, 0.f, stream, nullptr, low);
@@ -505,7 +527,10 @@ int launch_adapters(const l3ci_linear_args* a, const AdapterRows* low, cudaStrea
 
 }  // namespace
 
-int adapter_rows_launch(const l3ci_linear_args* a, const AdapterRows& low) {
+int adapter_rows_launch(const l3ci_linear_args* args, const AdapterRows& low) {
+  l3ci_linear_args with = *args, *a = &with;
+  a->groups = (int)((a->rows + L3CI_LINEAR_MAX_ROWS - 1) / L3CI_LINEAR_MAX_ROWS);
+  a->out_sg = L3CI_LINEAR_MAX_ROWS * a->out_st;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
   if (a->rows <= 8) return launch_adapters<8>(a, &low, stream);
   if (a->rows <= 16) return launch_adapters<16>(a, &low, stream);

@@ -16,7 +16,7 @@ struct AdapterRows {
   const __nv_bfloat16* b;
   int rank, adapters;
 };
-// l3ci_linear of up to L3CI_LINEAR_MAX_ROWS rows (one group, no activation, bf16) with these parts, one rounding.  The kernel ahead of it in the stream is to have
+// l3ci_linear of any number of rows (no activation, bf16) with these parts, one rounding.  The kernel ahead of it in the stream is to have
 // waited for its own predecessors before it lets this one start, and to leave z, index, x and w complete.
 int adapter_rows_launch(const l3ci_linear_args* a, const AdapterRows& low);
 
