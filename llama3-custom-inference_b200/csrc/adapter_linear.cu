@@ -12,18 +12,69 @@
 namespace l3ci {
 namespace {
 
+__device__ __forceinline__ int adapter_of(const l3ci_adapter_linear_args& p, long long row) {
+  const int id = row < p.rows ? __ldg(p.index + row) : -1;
+  return id >= 0 && id < p.adapters ? id : -1;
+}
+
+// The list of the adapters among 256 rows (linear_many.h), by all threads of a CTA of THREADS.
+template <int THREADS>
+__device__ void adapter_list(const l3ci_adapter_linear_args& p, int* list, int tile) {
+  __shared__ int ids[kAdapterTile], counts[kAdapterTile / 32];
+  constexpr int kRounds = kAdapterTile / THREADS;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) ids[k * THREADS + threadIdx.x] = adapter_of(p, (long long)tile * kAdapterTile + k * THREADS + threadIdx.x);
+  __syncthreads();
+  bool first[kRounds];                   // the first row of its adapter
+  unsigned mask[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int t = k * THREADS + threadIdx.x;
+    first[k] = ids[t] >= 0;
+    for (int i = 0; i < t && first[k]; ++i) first[k] = ids[i] != ids[t];
+    mask[k] = __ballot_sync(kFullMask, first[k]);
+    if (lane == 0) counts[t / 32] = __popc(mask[k]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int t = k * THREADS + threadIdx.x;
+    int at = __popc(mask[k] & ((1u << lane) - 1)), all = 0;
+    for (int w = 0; w < kAdapterTile / 32; ++w) {
+      if (w < t / 32) at += counts[w];
+      all += counts[w];
+    }
+    if (t == 0) list[0] = all;
+    if (!first[k]) continue;
+    int* entry = list + kAdapterHead + at * kAdapterEntry;
+    entry[0] = ids[t];
+    for (int w = 0; w < kAdapterTile / 32; ++w) {
+      unsigned others = 0;
+      for (int i = 0; i < 32; ++i) others |= (unsigned)(ids[w * 32 + i] != ids[t]) << i;
+      entry[4 + w] = (int)others;
+    }
+  }
+}
+
 // z[r, j] = scales[i] x[r] . a[i, j], i = index[r]; 0 without an adapter.  A CTA per row and kDots ranks, whose warps share the columns of K: a row of
 // x is read once for kDots rows of a, and a warp has all of its loads under way at once (a warp per r and j took 6.2 us for 64 rows of 8192
 // columns and rank 32, and slowed the product's weights, which stream meanwhile, by as much).
 constexpr int kDots = 4, kDotWarps = 4;
+constexpr int kDotRows = 512;   // up to which a row of a is read for every token (from L2) rather than for 32 at a time by few CTAs
 
-__global__ void __launch_bounds__(32 * kDotWarps) adapter_shrink_kernel(const l3ci_adapter_linear_args p, float* z) {
+__global__ void __launch_bounds__(32 * kDotWarps) adapter_shrink_kernel(const l3ci_adapter_linear_args p, float* z, int* lists) {
   __shared__ float parts[kDotWarps][kDots];
   pdl_wait();                // (before the next kernel may start: it reads x and w at once)
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.x, j0 = blockIdx.y * kDots, i = __ldg(p.index + r);
-  const bool has = i >= 0 && i < p.adapters;
+  const int r = blockIdx.x, j0 = blockIdx.y * kDots;
+  if (r >= p.rows) {         // (CTAs behind the rows, where the product is that of many rows)
+    if (j0 == 0) adapter_list<32 * kDotWarps>(p, lists + (r - p.rows) * kAdapterList, r - (int)p.rows);
+    return;
+  }
+  const int i = adapter_of(p, r);
+  const bool has = i >= 0;
   float s[kDots] = {};
   if (has) {
     const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + r * p.x_st;
@@ -60,7 +111,7 @@ __global__ void __launch_bounds__(32 * kDotWarps) adapter_shrink_kernel(const l3
 // The same of many rows, on the tensor cores: 32 rows of x a CTA, warps share the columns of K and add up at the end.  A dot product does not
 // ask in which order its terms come: a lane takes 8 neighbouring columns, 16 bytes, of a row of x and of a row of a, which are the operands of two
 // products.  Of every adapter among the 32 rows all rows' products are computed and its own rows' kept.
-// CTAs behind these list the adapters among every 256 rows (linear_many.h).
+// blockIdx.y: the ranks.  CTAs behind these make the lists.
 constexpr int kShrinkRows = 32, kShrinkWarps = 8;
 
 // NT: products of 8 ranks side by side.  (Two CTAs an SM: 6001 rows are then one wave.  16 warps at 128 registers, one CTA an SM, took 17.5 us for
@@ -69,44 +120,16 @@ template <int NT>
 __global__ void __launch_bounds__(32 * kShrinkWarps, 2) adapter_shrink_many_kernel(const l3ci_adapter_linear_args p, float* z, int* lists, int blocks) {
   constexpr int kShrinkRanks = 8 * NT;   // ranks at a time
   __shared__ float parts[kShrinkWarps][kShrinkRows][kShrinkRanks + 1];
-  __shared__ int ids[kAdapterTile];
+  __shared__ int ids[kShrinkRows];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-  auto id_of = [&](long long row) {
-    const int id = row < p.rows ? __ldg(p.index + row) : -1;
-    return id >= 0 && id < p.adapters ? id : -1;
-  };
-  if ((int)blockIdx.x >= blocks) {       // ---- a list ----
-    const int t = threadIdx.x, tile = blockIdx.x - blocks;
-    if (t < kAdapterTile) ids[t] = id_of((long long)tile * kAdapterTile + t);
-    __syncthreads();
-    bool first = t < kAdapterTile && ids[t] >= 0;            // the first row of its adapter
-    for (int i = 0; i < t && first; ++i) first = ids[i] != ids[t];
-    int* counts = reinterpret_cast<int*>(parts);
-    const unsigned mask = __ballot_sync(kFullMask, first);
-    if (lane == 0) counts[warp] = __popc(mask);
-    __syncthreads();
-    int at = __popc(mask & ((1u << lane) - 1)), all = 0;
-    for (int w = 0; w < kShrinkWarps; ++w) {
-      if (w < warp) at += counts[w];
-      all += counts[w];
-    }
-    int* list = lists + (long long)tile * kAdapterList;
-    if (t == 0) list[0] = all;
-    if (first) {
-      int* entry = list + kAdapterHead + at * kAdapterEntry;
-      entry[0] = ids[t];
-      for (int w = 0; w < kAdapterTile / 32; ++w) {
-        unsigned others = 0;
-        for (int i = 0; i < 32; ++i) others |= (unsigned)(ids[w * 32 + i] != ids[t]) << i;
-        entry[4 + w] = (int)others;
-      }
-    }
+  if ((int)blockIdx.x >= blocks) {
+    if (blockIdx.y == 0) adapter_list<32 * kShrinkWarps>(p, lists + (long long)(blockIdx.x - blocks) * kAdapterList, blockIdx.x - blocks);
     return;
   }
   const long long row0 = (long long)blockIdx.x * kShrinkRows;
-  if (threadIdx.x < kShrinkRows) ids[threadIdx.x] = id_of(row0 + threadIdx.x);
+  if (threadIdx.x < kShrinkRows) ids[threadIdx.x] = adapter_of(p, row0 + threadIdx.x);
   __syncthreads();
   const int mine = ids[lane];
   unsigned left = __ballot_sync(kFullMask, mine >= 0);     // rows whose adapters are still to come
@@ -121,7 +144,8 @@ __global__ void __launch_bounds__(32 * kShrinkWarps, 2) adapter_shrink_many_kern
     const unsigned here = __ballot_sync(kFullMask, mine == id);
     left &= ~here;
     const float scale = p.scales ? __ldg(p.scales + id) : 1.f;
-    for (int j0 = 0; j0 < p.rank; j0 += kShrinkRanks) {
+    {
+      const int j0 = blockIdx.y * kShrinkRanks;
       const int tiles = min(p.rank - j0, kShrinkRanks) / 8;
       const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + ((long long)id * p.rank + j0 + gid) * p.K + tig * 8;
       float acc[2][NT][4] = {};
@@ -226,16 +250,19 @@ extern "C" int l3ci_adapter_linear(const l3ci_adapter_linear_args* a) {
   l.K = a->K; l.N = a->N; l.groups = 1;
   l.stream = a->stream;
   const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(a->b);
-  if (few_rows(a)) {
-    L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)a->rows, (unsigned)(a->rank / kDots)), dim3(32 * kDotWarps), 0, stream, *a, z);
-    return adapter_rows_launch(&l, AdapterRows{z, a->index, b, a->rank, a->adapters});
-  }
+  const bool few = few_rows(a);
+  const long long blocks = (a->rows + kShrinkRows - 1) / kShrinkRows, tiles = few ? 0 : (a->rows + kAdapterTile - 1) / kAdapterTile;
   int* lists = reinterpret_cast<int*>(static_cast<uint8_t*>(a->scratch) + z_bytes(a));
-  const long long blocks = (a->rows + kShrinkRows - 1) / kShrinkRows, tiles = (a->rows + kAdapterTile - 1) / kAdapterTile;
-  auto shrink = [&](auto kernel) -> int {
-    L3CI_LAUNCH("adapter_shrink_many_kernel", kernel, dim3((unsigned)(blocks + tiles)), dim3(32 * kShrinkWarps), 0, stream, *a, z, lists, (int)blocks);
-    return L3CI_OK;
-  };
-  if (int st = a->rank <= 8 ? shrink(adapter_shrink_many_kernel<1>) : a->rank <= 16 ? shrink(adapter_shrink_many_kernel<2>) : shrink(adapter_shrink_many_kernel<4>)) return st;
+  if (a->rows <= kDotRows) {
+    L3CI_LAUNCH("adapter_shrink_kernel", adapter_shrink_kernel, dim3((unsigned)(a->rows + tiles), (unsigned)(a->rank / kDots)), dim3(32 * kDotWarps), 0, stream, *a, z, lists);
+  } else {
+    auto shrink = [&](auto kernel, int ranks) -> int {
+      const dim3 grid((unsigned)(blocks + tiles), (unsigned)((a->rank + ranks - 1) / ranks));
+      L3CI_LAUNCH("adapter_shrink_many_kernel", kernel, grid, dim3(32 * kShrinkWarps), 0, stream, *a, z, lists, (int)blocks);
+      return L3CI_OK;
+    };
+    if (int st = a->rank <= 8 ? shrink(adapter_shrink_many_kernel<1>, 8) : a->rank <= 16 ? shrink(adapter_shrink_many_kernel<2>, 16) : shrink(adapter_shrink_many_kernel<4>, 32)) return st;
+  }
+  if (few) return adapter_rows_launch(&l, AdapterRows{z, a->index, b, a->rank, a->adapters});
   return adapter_many_launch(&l, AdapterMany{z, b, lists, a->rank, a->adapters});
 }

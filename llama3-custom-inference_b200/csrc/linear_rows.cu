@@ -231,8 +231,12 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
           if (id[i] == id[i - 1]) v[i] = v[i - 1];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          const float4* zt = reinterpret_cast<const float4*>(z + (long long)min(tok0 + (i0 + i) * S, rows - 1) * d.rank + r);
-          const float4 z0 = __ldg(zt), z1 = __ldg(zt + 1);
+          const float4* zt = reinterpret_cast<const float4*>(z + (long long)(tok0 + (i0 + i) * S) * d.rank + r);
+          float4 z0 = make_float4(0.f, 0.f, 0.f, 0.f), z1 = z0;
+          if (id[i] >= 0) {                                    // (z of others may hold anything)
+            z0 = __ldg(zt);
+            z1 = __ldg(zt + 1);
+          }
           float f[8];
           unpack8(v[i], f);
           float& y = low[i0 + i];

@@ -85,6 +85,19 @@ def test_an_adapter_that_is_no_number_stays_with_its_rows(ext, device, rows):
     assert not torch.isfinite(got[2::3][:, 7]).any()
 
 
+@pytest.mark.parametrize("rows,K,N", [(5, 256, 128), (100, 256, 128), (600, 2048, 136), (1500, 256, 512)])
+def test_scratch_that_holds_no_numbers(ext, device, rows, K, N):
+    # rows without an adapter in every product's form: what their part of the scratch held before is nobody's
+    c = make(device, rows, K, N, 16, 3, [-1 if r % 3 == 0 else r % 2 for r in range(rows)], seed=rows)
+    want = ext.adapter_linear(**c)
+    check(want, c)
+    for _ in range(3):
+        held = [torch.full((n,), float("nan"), device=device) for n in (256, 4096, 65536, 1 << 20)]
+        torch.cuda.synchronize()
+        del held
+        assert torch.equal(ext.adapter_linear(**c), want)
+
+
 def test_shapes_strides_and_default_scales(ext, device):
     c = make(device, 24, 320, 144, 32, 5, spread(24, 5), seed=4)
     wide = torch.zeros(24, 400, dtype=BF16, device=device)

@@ -183,6 +183,16 @@ def test_two_graphs_at_once_and_lengths_that_change_between_replays(ext, device)
             check(out, case)
 
 
+def test_scratch_that_holds_no_numbers(ext, device):
+    case = attention_case([1, 40, 1, 2, 300], [3000, 900, 77, 5000, 1000], 8, 2, 128, 16, device, seed=1)
+    want = run(ext, case)
+    for _ in range(3):
+        held = [torch.full((n,), NAN, device=device) for n in (256, 65536, 1 << 20, 1 << 22, 12 << 20)]
+        torch.cuda.synchronize()
+        del held
+        assert torch.equal(run(ext, case), want)
+
+
 def test_empty_calls(ext, device):
     k = torch.zeros(4, 16, 2, 64, dtype=BF16, device=device)
     ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
