@@ -359,24 +359,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         for (int r = max(limit + 1 - j * kKeys, 0) + (warp - 2) * 32 + lane; r < kKeys; r += 64) {   // (keys up to `limit` all rows see)
           const bool behind = j * kKeys + r >= u.len;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kHalves * 8; c0 += 4) {
-            uint32_t w[4][4], at[4];
+          for (int c = 0; c < kHalves * 8; ++c) {      // (short loops here and in the output: unrolled code comes from memory every time)
+            const uint32_t at = v_smem + s * kTileBytes + (c >> 3) * kBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+            bool write = behind;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              at[c] = v_smem + s * kTileBytes + (c0 >> 3) * kBoxBytes + r * 128 + ((((c0 & 7) + c) ^ (r & 7)) << 4);
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3]) : "r"(at[c]) : "memory");
+            for (int x = 0; x < 4; ++x) {
+              if (behind) w[x] = 0;
+              if ((w[x] & 0x7f80u) == 0x7f80u) { w[x] &= 0xffff0000u; write = any = true; }
+              if ((w[x] & 0x7f800000u) == 0x7f800000u) { w[x] &= 0xffffu; write = any = true; }
             }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              bool write = behind;
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                if (behind) w[c][x] = 0;
-                if ((w[c][x] & 0x7f80u) == 0x7f80u) { w[c][x] &= 0xffff0000u; write = any = true; }
-                if ((w[c][x] & 0x7f800000u) == 0x7f800000u) { w[c][x] &= 0xffffu; write = any = true; }
-              }
-              if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at[c]), "r"(w[c][0]), "r"(w[c][1]), "r"(w[c][2]), "r"(w[c][3]) : "memory");
-            }
+            if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
           }
         }
         if (any) odd[segments % kMarks] = 1;
@@ -503,6 +497,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
     int g[2] = {0, 0}, mine[2] = {0, 0};
+    const int over_r = (65535 + p.R) / p.R;        // x * over_r >> 16 is x / R for the rows of a tile
     if (r == 0) {      // what the merge has to know of the unit that this run begins in the middle of
       Cut cut = {};
       if (begin < end && u.first + kUnitCost < begin) {
@@ -532,7 +527,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const float inv = lm.x == 0.f ? 0.f : 1.f / lm.x;
         float* rec = part_of<D>(p, part, j0 == 0);
         const uint32_t to = t_o[e] + lane_addr;
-        if (taken) {
+        if (__builtin_expect(taken, 0)) {
           // values that the guards took out, for the rows that see them: from the cache, key by key, into O_e (a call with such values is lost anyway)
           const int upto = r < tokens * p.R ? min(min(first_limit(u, e) + r / p.R, u.len - 1), j1 * kKeys - 1) : -1;
 #pragma unroll 1
@@ -574,24 +569,23 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 #pragma unroll 1
           for (int h = 0; h < kHalves; ++h) {
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-              uint32_t y[32];
-              tmem_ld32(to + h * 64 + c * 32, y);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t y[16];
+              tmem_ld16(to + h * 64 + c * 16, y);
               tc_wait_ld();
-              uint4* dst = reinterpret_cast<uint4*>(stage + lane * kPitch + c * 64);
+              float f[8];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t w[4];
+              for (int v = 0; v < 2; ++v) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(y[8 * q + 2 * i]) * inv, __uint_as_float(y[8 * q + 2 * i + 1]) * inv);
-                dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(y[8 * v + i]) * inv;
+                *reinterpret_cast<uint4*>(stage + lane * kPitch + c * 32 + v * 16) = pack8(f);
               }
             }
             if (h == kHalves - 1) read();
             __syncwarp();
-#pragma unroll 2
+#pragma unroll 1
             for (int i = 0; i < 8; ++i) {
-              const int row = i * 4 + (lane >> 3), t = (q4 * 32 + row) / p.R;
+              const int row = i * 4 + (lane >> 3), t = (q4 * 32 + row) * over_r >> 16;
               if (t < tokens)
                 *reinterpret_cast<uint4*>(out + (t0 + t) * a.o_st + (q4 * 32 + row - t * p.R) * a.o_sh + h * 64) =
                     *reinterpret_cast<const uint4*>(stage + row * kPitch + (lane & 7) * 16);
@@ -600,14 +594,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
         } else {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t y[32];
-            tmem_ld32(to + c * 32, y);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t y[16];
+            tmem_ld16(to + c * 16, y);
             tc_wait_ld();
-            if (c == D / 32 - 1) read();
+            if (c == D / 16 - 1) read();
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<uint4*>(rec + ((long long)(c * 8 + q) * (2 * kRows) + e * kRows + r) * 4) = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(rec + ((long long)(c * 4 + q) * (2 * kRows) + e * kRows + r) * 4) = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
           }
           rec[2 * kRows * D + e * kRows + r] = lm.y;
           rec[2 * kRows * (D + 1) + e * kRows + r] = lm.x;
