@@ -34,12 +34,15 @@ constexpr int kKeys = 128;     // keys of a tile
 constexpr int kStages = 2;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kThreads = 32 * (4 + kSoftmaxWarps + 4);
+constexpr int kReaders = 1 + 2 + kSoftmaxWarps + 4;            // warps that read the segments
 constexpr int kRegsLow = 56, kRegsHigh = 192, kRegsOut = 72;   // of the producer's, the softmax and the output warpgroups
 static_assert(4 * kRegsLow + kSoftmaxWarps * kRegsHigh + 4 * kRegsOut <= 16 * 128, "register re-deal");
 constexpr uint32_t kTmemCols = 512;                            // S_0, S_1 (128 columns each), O_0, O_1 (D columns each)
-constexpr int kMarks = 4;      // the guards are at most three segments ahead of the output (one-tile segments: two in the ring of V, one on its way out)
+constexpr int kSegments = 8;   // of the ring (the guards are at most three ahead of the output: one-tile segments, two in the ring of V, one on its way out)
 constexpr int kMergeThreads = 256;
-constexpr int kUnitCost = 1;                                   // columns that a unit counts beside its tiles: its start and its end
+// Columns that a tile counts in the deal, and a unit beside its tiles: its start and its end.
+constexpr int kTileCost = 2;
+constexpr int unit_cost(int D) { return D == 128 ? 2 : 1; }
 constexpr int kMergeItems = 4;                                 // float4 a thread merges
 
 // The unit that part g of the deal begins in the middle of, written by its CTA for the merge; parts 0: none, or its first cut is another part's.
@@ -69,9 +72,14 @@ __device__ __forceinline__ int unit_tiles(const PagedSeq& s, int m, int block) {
   return seen <= 0 ? 1 : (seen + kKeys - 1) / kKeys;
 }
 
-// A run of keys' tiles of a unit; first: the unit's first column.
-struct Unit {
-  int b, h, m, n, len, first, tiles;
+// What a CTA does next: tiles [j0, j1) of a unit's keys; j1 0: nothing is left.  The producer walks through the deal and leaves these in a ring for
+// the other warps, whose code has to be short.
+struct Segment {
+  int j0, j1, ne;      // ne: tiles of rows, 1 or 2
+  int limit;           // last key that the unit's first token sees
+  int len, b, h;
+  int t0, n, row;      // the unit's first token, the sequence's tokens, its row in packed tensors
+  int whole, pad;
 };
 
 template <int D>
@@ -94,20 +102,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   // as in prefill_tc_persist_kernel; V_OK: the guard warps have been through the tile, if it is one of theirs
   // (they arrive on V_EMPTY too, so that they never miss a phase of V_FULL)
   enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_OK = 14, P_FULL = 16, L_FULL = 18, O_READ = 20,
-         N_BARS = 22 };
+         SEG_FULL = 22, SEG_EMPTY = SEG_FULL + kSegments, N_BARS = SEG_EMPTY + kSegments };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
-  int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kMarks]: values taken out of tiles of a segment
-  int* sums = odd + kMarks;                                            // [16 warps]
+  int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kSegments]: values taken out of tiles of a segment
+  int* sums = odd + kSegments;                                            // [16 warps]
   float* stat = reinterpret_cast<float*>(sums + 16);               // [2 tiles][128 rows][l, m_ref]
-  Unit* units = reinterpret_cast<Unit*>(stat + 4 * kRows);         // [16 warps]: where each is (registers are few)
-  int* pref = reinterpret_cast<int*>(units + 16);                  // [B + 1]
+  Segment* segs = reinterpret_cast<Segment*>(stat + 4 * kRows);    // [kSegments]
+  int* pref = reinterpret_cast<int*>(segs + kSegments);            // [B + 1]
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_FULL ? kSoftmaxWarps / 2 : i >= V_OK ? 2 : i == V_EMPTY || i == V_EMPTY + 1 ? 3 : 1);
-    for (int i = 0; i < kMarks; ++i) odd[i] = 0;
+    for (int i = 0; i < N_BARS; ++i)
+      mbar_init(bar(i), i >= SEG_EMPTY ? kReaders : i >= SEG_FULL ? 1 : i >= P_FULL ? kSoftmaxWarps / 2 : i >= V_OK ? 2 : i == V_EMPTY || i == V_EMPTY + 1 ? 3 : 1);
+    for (int i = 0; i < kSegments; ++i) odd[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
@@ -119,11 +128,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     tmem_relinquish();
   }
   pdl_wait();
-  // ---- columns (kUnitCost and a tile of keys each of every unit) before every sequence ----
+  // ---- columns of the deal before every sequence ----
+  constexpr int kUnitCost = unit_cost(D);
   const int block = 2 * cp.tile_tokens;
   auto columns_of_head = [&](const PagedSeq& s) {
     int sum = 0;
-    for (int m = 0; m * block < s.n; ++m) sum += kUnitCost + unit_tiles(s, m, block);
+    for (int m = 0; m * block < s.n; ++m) sum += kUnitCost + kTileCost * unit_tiles(s, m, block);
     return sum;
   };
   {
@@ -154,78 +164,111 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_s[2] = {tmem, tmem + 128u};
   const uint32_t t_o[2] = {tmem + 256u, tmem + 256u + (uint32_t)D};
-  const int total = pref[a.B], parts = min(total, p.max_parts), part = blockIdx.x;
-  const int begin = part < parts ? fd_range_begin(part, total, parts) : 0, end = part < parts ? fd_range_begin(part + 1, total, parts) : 0;
+  const int total = pref[a.B], parts = max(min(total / kTileCost, p.max_parts), 1), part = blockIdx.x;   // (no run between two tiles' first columns)
+  const int begin = total > 0 && part < parts ? fd_range_begin(part, total, parts) : 0, end = total > 0 && part < parts ? fd_range_begin(part + 1, total, parts) : 0;
 
-  // ---- a CTA's run is a list of segments: tiles [j0, j1) of a unit ----
-  auto unit_at = [&](int col) {                         // the unit that holds a column
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pref[mid] <= col) lo = mid; else hi = mid;
-    }
-    Unit u;
-    u.b = lo;
-    const PagedSeq s = paged_seq(p, lo);
-    u.n = s.n;
-    u.len = s.len;
-    const int per_head = (pref[lo + 1] - pref[lo]) / a.Hkv, local = col - pref[lo];
-    u.h = local / per_head;
-    int before = u.h * per_head;
-    for (u.m = 0;; ++u.m) {
-      u.tiles = unit_tiles(s, u.m, block);
-      if (before + kUnitCost + u.tiles > local) break;
-      before += kUnitCost + u.tiles;
-    }
-    u.first = pref[lo] + before;
-    return u;
+  // the next segment; false: the wait for it ran out
+  auto take = [&](int k) {
+    __syncwarp();
+    if (k > 0 && lane == 0) mbar_arrive(bar(SEG_EMPTY + (k - 1) % kSegments));
+    return mbar_wait_bounded(bar(SEG_FULL + k % kSegments), (k / kSegments) & 1);
   };
-  auto next_unit = [&](Unit& u) {
-    u.first += kUnitCost + u.tiles;
-    if (++u.m * block >= u.n) {
-      u.m = 0;
-      if (++u.h == a.Hkv) {
-        u.h = 0;
-        do ++u.b; while (u.b < a.B && pref[u.b + 1] == pref[u.b]);
-        if (u.b >= a.B) return;
-        const PagedSeq s = paged_seq(p, u.b);
-        u.n = s.n;
-        u.len = s.len;
-      }
-    }
-    u.tiles = unit_tiles(PagedSeq{u.n, u.len}, u.m, block);
-  };
-  auto tiles_from = [&](const Unit& u, int col) { return max(col - u.first - kUnitCost, 0); };
-  auto tiles_to = [&](const Unit& u) { return max(min(u.tiles, end - u.first - kUnitCost), 0); };
-  // to the unit behind u, whose tiles up to j1 have been dealt with; false: the run ends
-  auto next_segment = [&](Unit& u, int j1) {
-    if (j1 < u.tiles) return false;
-    next_unit(u);
-    return u.first + kUnitCost < end;
-  };
-  auto both = [&](const Unit& u) { return u.m * block + cp.tile_tokens < u.n; };      // the second tile of rows has tokens
-  auto first_limit = [&](const Unit& u, int e) { return u.len - u.n + u.m * block + e * cp.tile_tokens; };   // last key of the tile's first token
   auto cut_tile = [&](int j, int limit) { return j * kKeys + kKeys - 1 > limit; };    // some row does not see all keys
   bool ok = true;
   int fill = 0;        // tiles of keys so far: stage and phase of the rings follow
-  Unit& u = units[warp];
-  u = begin < end ? unit_at(begin) : Unit{};
-  bool on = tiles_to(u) > tiles_from(u, begin);   // there is something to do
   int segments = 0;
 
   if (warp == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
-    // ---- producer: lane 0 the query rows, every lane the tokens of its own copies ----
+    // ---- producer: deals the segments; lane 0 copies the query rows, every lane the tokens of its own copies ----
+    struct Unit { int b, h, m, n, len, first, tiles; };   // first: its first column
+    auto unit_at = [&](int col) {                         // the unit that holds a column
+      int lo = 0, hi = a.B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pref[mid] <= col) lo = mid; else hi = mid;
+      }
+      Unit u;
+      u.b = lo;
+      const PagedSeq s = paged_seq(p, lo);
+      u.n = s.n;
+      u.len = s.len;
+      const int per_head = (pref[lo + 1] - pref[lo]) / a.Hkv, local = col - pref[lo];
+      u.h = local / per_head;
+      int before = u.h * per_head;
+      for (u.m = 0;; ++u.m) {
+        u.tiles = unit_tiles(s, u.m, block);
+        if (before + kUnitCost + kTileCost * u.tiles > local) break;
+        before += kUnitCost + kTileCost * u.tiles;
+      }
+      u.first = pref[lo] + before;
+      return u;
+    };
+    auto next_unit = [&](Unit& u) {
+      u.first += kUnitCost + kTileCost * u.tiles;
+      if (++u.m * block >= u.n) {
+        u.m = 0;
+        if (++u.h == a.Hkv) {
+          u.h = 0;
+          do ++u.b; while (u.b < a.B && pref[u.b + 1] == pref[u.b]);
+          if (u.b >= a.B) return;
+          const PagedSeq s = paged_seq(p, u.b);
+          u.n = s.n;
+          u.len = s.len;
+        }
+      }
+      u.tiles = unit_tiles(PagedSeq{u.n, u.len}, u.m, block);
+    };
+    // (a tile is dealt with its first column)
+    auto tiles_from = [&](const Unit& u, int col) { return max(col - u.first - kUnitCost + kTileCost - 1, 0) / kTileCost; };
+    Unit u = {}, held = {};
+    int col = begin;
+    bool on = begin < end, waits = false, last = false;    // the run's first unit's part is still to come; it is at work
+    if (on) {
+      u = unit_at(begin);
+      if (tiles_from(u, begin) == u.tiles) next_unit(u);
+      on = u.first + kUnitCost < end && tiles_from(u, end) > tiles_from(u, begin);
+    }
+    if (lane == 0) {      // what the merge has to know of a unit that this run begins in the middle of
+      Cut cut = {};
+      if (on && u.first + kUnitCost < begin) {
+        cut.first = fd_cta_of(u.first + kUnitCost, total, parts);
+        if (cut.first == part - 1) {
+          cut.b = u.b;
+          cut.h = u.h;
+          cut.m = u.m;
+          cut.last = fd_cta_of(u.first + kUnitCost + kTileCost * (u.tiles - 1), total, parts);
+          cut.parts = cut.last - cut.first + 1;
+        }
+      }
+      cp.cuts[part] = cut;
+    }
+    // Such a part is taken last: the runs of one head then start at its first keys together and go through them side by side, and K and V come
+    // from memory about once (in the order of the deal they came six times: 907 MB instead of 135 for 2 x 512 tokens of 16500 keys).
+    if (on && u.first + kUnitCost < begin && u.first + 2 * kUnitCost + kTileCost * u.tiles < end) {
+      held = u;
+      waits = true;
+      next_unit(u);
+      col = u.first;
+    }
     const uint64_t policy = l2_evict_first_policy();
     const int copies = kKeys / cp.box;                      // per half of a tile
-    for (int col = begin; on && ok; ++segments) {
+    for (;; ++segments) {
+      const int slot = segments % kSegments;
+      if (segments >= kSegments && !mbar_wait_bounded(bar(SEG_EMPTY + slot), (segments / kSegments - 1) & 1)) { ok = false; break; }
+      const int j0 = tiles_from(u, col), j1 = on ? min(u.tiles, tiles_from(u, end)) : 0;
+      const int row = a.starts && on ? __ldg(a.starts + u.b) : 0;
+      const bool two = (u.m * 2 + 1) * cp.tile_tokens < u.n;
+      if (lane == 0) {
+        segs[slot] = Segment{j0, j1, two ? 2 : 1, u.len - u.n + u.m * block, u.len, u.b, u.h, u.m * block, u.n, row, j0 == 0 && j1 == u.tiles, 0};
+        mbar_arrive(bar(SEG_FULL + slot));
+      }
+      if (!on) break;
       auto page_of = [&](int j) {                          // of this lane's tokens of tile j; one past the last: nothing is there
         const int token = j * kKeys + lane * cp.box;
         const int page = lane < copies && token < u.len ? __ldg(a.page_table + u.b * a.table_st + token / a.page_size) : -1;
         return page >= 0 && page < a.pages ? page : (int)a.pages;
       };
-      const int j0 = tiles_from(u, col), j1 = tiles_to(u);
-      const int row = (a.starts ? __ldg(a.starts + u.b) : 0) + u.m * block;
       int page = page_of(j0);
       for (int j = j0; j < j1 && ok; ++j, ++fill) {
         const int s = fill % kStages, off = (j * kKeys + lane * cp.box) % a.page_size;
@@ -243,20 +286,33 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (j == j0) {     // (behind the first keys, whose place is free before the last unit's scores are done)
           if (segments > 0 && !mbar_wait_bounded(bar(Q_EMPTY), (segments - 1) & 1)) { ok = false; break; }
           if (lane == 0) {
-            const int tiles = both(u) ? 2 : 1;
+            const int tiles = two ? 2 : 1;
             mbar_expect_tx(bar(Q_FULL), tiles * kHalves * cp.tile_tokens * p.R * 128);
             for (int e = 0; e < tiles; ++e)
 #pragma unroll
               for (int h = 0; h < kHalves; ++h)
-                tma_load_4d(q_smem + e * kTileBytes + h * kBoxBytes, &qmap, bar(Q_FULL), h * 64, u.h * p.R, row + e * cp.tile_tokens, a.starts ? 0 : u.b, policy);
+                tma_load_4d(q_smem + e * kTileBytes + h * kBoxBytes, &qmap, bar(Q_FULL), h * 64, u.h * p.R, row + u.m * block + e * cp.tile_tokens, a.starts ? 0 : u.b, policy);
           }
         }
         if (fill >= kStages && !mbar_wait_bounded(bar(V_EMPTY + s), par)) { ok = false; break; }
         load(vmap, v_smem, bar(V_FULL + s));
         page = ahead;
       }
-      on = next_segment(u, j1);
-      col = u.first;
+      if (!ok) break;
+      on = false;
+      if (!last) {                       // to the unit behind it, or to the part that waits
+        if (j1 == u.tiles) {
+          next_unit(u);
+          col = u.first;
+          on = u.first + kUnitCost < end;
+        }
+        if (!on && waits) {
+          u = held;
+          col = begin;
+          on = last = true;
+          waits = false;
+        }
+      }
     }
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
@@ -271,7 +327,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     // once, and there is one place for each product's code (what is unrolled further falls out of the instruction cache that the warp shares with
     // the softmax: with both tiles of rows and both stages unrolled a tile of keys took 3.3 us instead of 2.7).
     uint32_t p_phase = 0, o_phase = 0, o_used = 0, guarded = 0;   // phases of P_FULL, O_READ and V_OK, a bit for each; whether O_e has been used
-    int nj = tiles_from(u, begin), nj1 = tiles_to(u), nne = both(u) ? 2 : 1, nlimit = first_limit(u, 0);   // the tile whose scores come
+    ok = take(0);
+    int nj = segs[0].j0, nj1 = ok ? segs[0].j1 : 0, nne = segs[0].ne, nlimit = segs[0].limit;   // the tile whose scores come
+    bool on = nj1 > 0;
     int j = 0, ne = 0, limit = 0;                                 // the tile whose values come: the one before; ne 0: none
     bool first = true, nfirst = true;
     for (fill = -1; (on || ne > 0) && ok; ++fill) {
@@ -331,23 +389,25 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       first = nfirst;
       nfirst = false;
       if (on && ++nj == nj1) {
-        on = next_segment(u, nj1);
-        if (on) {
-          nfirst = true;
-          ++segments;
-          nj = 0;
-          nj1 = tiles_to(u);
-          nne = both(u) ? 2 : 1;
-          nlimit = first_limit(u, 0);
-        }
+        if (!take(++segments)) { ok = false; break; }
+        const Segment& g = segs[segments % kSegments];
+        nj1 = g.j1;
+        on = nj1 > 0;
+        nfirst = true;
+        nj = g.j0;
+        nne = g.ne;
+        nlimit = g.limit;
       }
     }
   } else if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
     // ---- guards: a key's values a thread, tiles at the diagonal and the end only ----
-    for (int col = begin; on && ok; ++segments) {
-      const int j1 = tiles_to(u), limit = first_limit(u, 0);
-      for (int j = tiles_from(u, col); j < j1 && ok; ++j, ++fill) {
+    for (; ok; ++segments) {
+      if (!take(segments)) { ok = false; break; }
+      const Segment& g = segs[segments % kSegments];
+      const int j1 = g.j1, limit = g.limit, len = g.len;
+      if (j1 == 0) break;
+      for (int j = g.j0; j < j1 && ok; ++j, ++fill) {
         const int s = fill % kStages;
         if (!mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
         if (!cut_tile(j, limit)) {
@@ -357,7 +417,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         bool any = false;
 #pragma unroll 1
         for (int r = max(limit + 1 - j * kKeys, 0) + (warp - 2) * 32 + lane; r < kKeys; r += 64) {   // (keys up to `limit` all rows see)
-          const bool behind = j * kKeys + r >= u.len;
+          const bool behind = j * kKeys + r >= len;
 #pragma unroll 1
           for (int c = 0; c < kHalves * 8; ++c) {      // (short loops here and in the output: unrolled code comes from memory every time)
             const uint32_t at = v_smem + s * kTileBytes + (c >> 3) * kBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -373,7 +433,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
           }
         }
-        if (any) odd[segments % kMarks] = 1;
+        if (any) odd[segments % kSegments] = 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -381,8 +441,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           mbar_arrive(bar(V_EMPTY + s));
         }
       }
-      on = next_segment(u, j1);
-      col = u.first;
     }
   } else if (warp < 4 + kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
@@ -393,10 +451,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     constexpr float kLazy = 8.f;                   // log2 of how far the running maximum may outgrow m_ref
     const int token = r / p.R;                     // of the tile
     int g = 0, mine = 0;                           // tiles and segments of this group so far
-    for (int col = begin; on && ok; ++segments) {
-      const int j0 = tiles_from(u, col), j1 = tiles_to(u);
-      if (e == 0 || both(u)) {
-        const int limit0 = first_limit(u, e), limit = token < cp.tile_tokens ? limit0 + token : -1;   // last key this row may see
+    for (; ok; ++segments) {
+      if (!take(segments)) { ok = false; break; }
+      const Segment& s = segs[segments % kSegments];
+      const int j0 = s.j0, j1 = s.j1;
+      if (j1 == 0) break;
+      if (e < s.ne) {
+        const int limit0 = s.limit + e * cp.tile_tokens;
+        const int limit = token < cp.tile_tokens ? min(limit0 + token, s.len - 1) : -1;   // last key this row may see
         float m_ref = -INFINITY, l_run = 0.f;
         for (int j = j0; j < j1 && ok; ++j, ++g) {
           if (!mbar_wait_bounded(bar(S_FULL + e), g & 1)) { ok = false; break; }
@@ -406,7 +468,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, x[c]);
           tc_wait_ld();
           if (__builtin_expect(cut_tile(j, limit0), 0)) {
-            const int left = min(limit, u.len - 1) - j * kKeys;    // last key of the tile that this row sees
+            const int left = limit - j * kKeys;                    // last key of the tile that this row sees
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -488,8 +550,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (lane == 0) mbar_arrive(bar(L_FULL + e));
         ++mine;
       }
-      on = next_segment(u, j1);
-      col = u.first;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOut));
@@ -498,48 +558,37 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
     int g[2] = {0, 0}, mine[2] = {0, 0};
     const int over_r = (65535 + p.R) / p.R;        // x * over_r >> 16 is x / R for the rows of a tile
-    if (r == 0) {      // what the merge has to know of the unit that this run begins in the middle of
-      Cut cut = {};
-      if (begin < end && u.first + kUnitCost < begin) {
-        cut.first = fd_cta_of(u.first + kUnitCost, total, parts);
-        if (cut.first == part - 1) {
-          cut.b = u.b;
-          cut.h = u.h;
-          cut.m = u.m;
-          cut.last = fd_cta_of(u.first + kUnitCost + u.tiles - 1, total, parts);
-          cut.parts = cut.last - cut.first + 1;
-        }
-      }
-      cp.cuts[part] = cut;
-    }
-    for (int col = begin; on && ok; ++segments) {
-      const int j0 = tiles_from(u, col), j1 = tiles_to(u), ne = both(u) ? 2 : 1;
-      const bool whole = j0 == 0 && j1 == u.tiles;
-      const long long row0 = paged_row0(p, u.b, a.o_sb, a.o_st);
+    for (; ok; ++segments) {
+      if (!take(segments)) { ok = false; break; }
+      const Segment& s = segs[segments % kSegments];
+      const int j0 = s.j0, j1 = s.j1, ne = s.ne;
+      if (j1 == 0) break;
+      const bool whole = s.whole != 0;
+      const long long row0 = a.starts ? s.row * a.o_st : s.b * a.o_sb;
       for (int e = 0; e < ne && ok; ++e) {
         if (!mbar_wait_bounded(bar(L_FULL + e), mine[e] & 1)) { ok = false; break; }
         const float2 lm = *reinterpret_cast<const float2*>(stat + (e * kRows + r) * 2);
         g[e] += j1 - j0;
         if (!mbar_wait_bounded(bar(O_FULL + e), (g[e] - 1) & 1)) { ok = false; break; }   // the segment's last product
         tc_fence_after();
-        const int t0 = u.m * block + e * cp.tile_tokens, tokens = min(cp.tile_tokens, u.n - t0);   // tokens of the tile
-        const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kMarks) != 0;
+        const int t0 = s.t0 + e * cp.tile_tokens, tokens = min(cp.tile_tokens, s.n - t0);   // tokens of the tile
+        const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kSegments) != 0;
         const float inv = lm.x == 0.f ? 0.f : 1.f / lm.x;
         float* rec = part_of<D>(p, part, j0 == 0);
         const uint32_t to = t_o[e] + lane_addr;
         if (__builtin_expect(taken, 0)) {
           // values that the guards took out, for the rows that see them: from the cache, key by key, into O_e (a call with such values is lost anyway)
-          const int upto = r < tokens * p.R ? min(min(first_limit(u, e) + r / p.R, u.len - 1), j1 * kKeys - 1) : -1;
+          const int upto = r < tokens * p.R ? min(min(s.limit + e * cp.tile_tokens + r / p.R, s.len - 1), j1 * kKeys - 1) : -1;
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t y[16];
             tmem_ld16(to + c, y);
             tc_wait_ld();
 #pragma unroll 1
-            for (int key = max(max(j0 * kKeys, first_limit(u, 0) + 1), 0); key <= upto; ++key) {
-              const int page = __ldg(a.page_table + u.b * a.table_st + key / a.page_size);
+            for (int key = max(max(j0 * kKeys, s.limit + 1), 0); key <= upto; ++key) {
+              const int page = __ldg(a.page_table + s.b * a.table_st + key / a.page_size);
               if (page < 0 || page >= a.pages) continue;
-              const uint16_t* v = static_cast<const uint16_t*>(a.cache_v) + page * a.cache_sp + key % a.page_size * a.cache_st + u.h * D + c;
+              const uint16_t* v = static_cast<const uint16_t*>(a.cache_v) + page * a.cache_sp + key % a.page_size * a.cache_st + s.h * D + c;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const uint32_t w = __ldg(v + i);
@@ -554,7 +603,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         auto read = [&]() {                                   // O_e and the row's sums are in registers: they may take the next segment's
           if (e == ne - 1) {
             asm volatile("bar.sync 2, 128;" ::: "memory");    // (all have read the mark)
-            if (r == 0) odd[segments % kMarks] = 0;
+            if (r == 0) odd[segments % kSegments] = 0;
           }
           tc_fence_before();
           __syncwarp();
@@ -565,7 +614,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           uint8_t* stage = stage_all + q4 * (2 * kRows * kSPitch / 4);
           constexpr int kPitch = 128 + 16;
           static_assert(32 * kPitch <= 2 * kRows * kSPitch / 4, "staging rows of a warp");
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 + (long long)(u.h * p.R) * a.o_sh + (lane & 7) * 8;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 + (long long)(s.h * p.R) * a.o_sh + (lane & 7) * 8;
 #pragma unroll 1
           for (int h = 0; h < kHalves; ++h) {
 #pragma unroll 1
@@ -608,8 +657,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         ++mine[e];
       }
-      on = next_segment(u, j1);
-      col = u.first;
     }
   }
   if (!ok && lane == 0 && a.status) atomicExch(a.status, (int)L3CI_ERR_DEVICE_WAIT);
@@ -694,14 +741,14 @@ __global__ void __launch_bounds__(kMergeThreads) paged_chunk_merge_kernel(const 
 // ---- host ----
 size_t chunk_smem(int D, int B) {
   const size_t tile = (size_t)(D / 64) * 128 * 128;
-  return 1024 + 6 * tile + 2 * kRows * 80 + 23 * 8 + (kMarks + 16) * 4 + 4 * kRows * 4 + 16 * sizeof(Unit) + (size_t)(B + 1) * 4;
+  return 1024 + 6 * tile + 2 * kRows * 80 + (23 + 2 * kSegments) * 8 + (kSegments + 16) * 4 + 4 * kRows * 4 + kSegments * sizeof(Segment) + (size_t)(B + 1) * 4;
 }
 
 int chunk_parts(const PagedParams& p) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
   // (columns at most: every token's own unit of all the keys that the table can hold)
   const long long rows = p.a.starts ? p.a.rows : (long long)p.a.B * p.a.T, block = 2 * (kRows / p.R);
-  const long long columns = (rows / block + p.a.B) * p.a.Hkv * (((long long)p.cap + kKeys - 1) / kKeys + 1 + kUnitCost);
+  const long long columns = (rows / block + p.a.B) * p.a.Hkv * (((long long)p.cap + kKeys - 1) / kKeys + 1 + unit_cost(p.a.D));
   return (int)(columns < sms ? columns : sms);
 }
 
