@@ -17,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "bf16x8.cuh"
 #include "flash_decode_plan.h"
 #include "host_common.h"
@@ -414,19 +416,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const PagedPara
   cp_async_wait<0>();
 }
 
-// Merges the parts of the units that were cut.  D / 4 lanes per query row and group of parts, `groups` (a power of two) groups of parts per row.
+// Merges the parts of the units of few rows that were cut.  D / 4 lanes per query row and group of parts, `groups` (a power of two) groups of parts
+// per row.
 template <int D, int NB>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedParams p, int groups, int row_slots) {
+__device__ __forceinline__ void merge_rows(const PagedParams& p, int groups, int row_slots, int cta) {
   constexpr int kTile = fd_tile_tokens(D), kLanes = D / 4, kSets = kMergeThreads / kLanes;
   __shared__ float4 sums[kSets][kLanes];
   __shared__ float2 stats[kSets];
   const l3ci_paged_attention_args& a = p.a;
   const int set = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, group = set & (groups - 1);
-  const long long item = (long long)blockIdx.x * (kSets / groups) + set / groups;
+  const long long item = (long long)cta * (kSets / groups) + set / groups;
   const long long unit = item / row_slots;
   const int row = (int)(item - unit * row_slots), b = (int)(unit / a.Hkv), h = (int)(unit - (long long)b * a.Hkv);
-  pdl_wait();
-  pdl_launch_dependents();
   bool live = b < a.B;
   const PagedSeq s = live ? paged_seq(p, b) : PagedSeq{0, 0};
   live = live && row < s.n * p.R;
@@ -505,6 +506,82 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedP
   *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
+// Puts the parts of a cut unit of a chunk together: kShares CTAs for every part of the deal, each with a share of the unit's rows and columns.
+constexpr int kMergeItems = 4;       // float4 a thread merges
+template <int D>
+constexpr int kShares = 2 * kChunkRows * (D / 4) / (kMergeThreads * kMergeItems);
+
+template <int D>
+__device__ __forceinline__ void merge_chunk(const ChunkParams& cp, int cta) {
+  const PagedParams& p = cp.p;
+  const l3ci_paged_attention_args& a = p.a;
+  const int4 c0 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + cta / kShares<D> + 1)), c1 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + cta / kShares<D> + 1) + 1);
+  const int b = c0.x, h = c0.y, m = c0.z, first = c0.w, parts = c1.y;
+  if (parts < 2) return;
+  const PagedSeq s = paged_seq(p, b);
+  const int t_unit = m * 2 * cp.tile_tokens;
+  const long long row0 = paged_row0(p, b, a.o_sb, a.o_st);
+  // neighbouring lanes: 8 rows of 4 vectors each (runs of 128 bytes of a part, of 32 bytes of the result)
+  constexpr int kPerRow = D / 4;
+#pragma unroll 1
+  for (int i = 0; i < kMergeItems; ++i) {
+    const int item = (cta % kShares<D> * kMergeItems + i) * kMergeThreads + threadIdx.x;
+    const int in8 = item & 31, rest = item >> 5;
+    const int vec = (rest % (kPerRow / 4)) * 4 + (in8 >> 3), row = rest / (kPerRow / 4) * 8 + (in8 & 7);   // row: 0 .. 255
+    const int e = row / kChunkRows, t = (row % kChunkRows) / p.R, token = t_unit + e * cp.tile_tokens + t;
+    if (t >= cp.tile_tokens || token >= s.n) continue;
+    float mx = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAtOnce = 4;
+    for (int p0 = 0; p0 < parts; p0 += kAtOnce) {
+      float mv[kAtOnce], lv[kAtOnce];
+      float4 ov[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        mv[k] = -INFINITY;
+        lv[k] = 0.f;
+        ov[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p0 + k < parts) {
+          const float* rec = chunk_part_of<D>(p, first + p0 + k, p0 + k == 0);
+          ov[k] = __ldcg(reinterpret_cast<const float4*>(rec) + vec * (2 * kChunkRows) + row);
+          mv[k] = __ldcg(rec + 2 * kChunkRows * D + row);
+          lv[k] = __ldcg(rec + 2 * kChunkRows * (D + 1) + row);
+        }
+      }
+      float mn = mx;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, mv[k]);
+      const float mu = mn == -INFINITY ? 0.f : mn, w0 = fast_exp2(mx - mu);
+      l *= w0;
+      acc.x *= w0; acc.y *= w0; acc.z *= w0; acc.w *= w0;
+      mx = mn;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        if (p0 + k >= parts) break;
+        const float w = fast_exp2(mv[k] - mu);
+        l = fmaf(lv[k], w, l);
+        acc.x = fmaf(ov[k].x, w, acc.x);
+        acc.y = fmaf(ov[k].y, w, acc.y);
+        acc.z = fmaf(ov[k].z, w, acc.z);
+        acc.w = fmaf(ov[k].w, w, acc.w);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 + token * a.o_st + (long long)(h * p.R + row % kChunkRows - t * p.R) * a.o_sh;
+    *reinterpret_cast<uint2*>(out + vec * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  }
+}
+
+// NB 0: no sequences of few rows.  The first rows_ctas CTAs are theirs.
+template <int D, int NB>
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedParams p, int groups, int row_slots, int rows_ctas, const ChunkParams cp) {
+  pdl_wait();
+  pdl_launch_dependents();
+  if constexpr (NB > 0)
+    if ((int)blockIdx.x < rows_ctas) return merge_rows<D, NB>(p, groups, row_slots, blockIdx.x);
+  merge_chunk<D>(cp, blockIdx.x - rows_ctas);
+}
+
 // The arguments of a call, checked; kNothing: there is nothing to do.
 constexpr int kNothing = -1;
 int check(const l3ci_paged_attention_args* a) {
@@ -548,30 +625,47 @@ RowsPlan rows_plan(const PagedParams& p) {
   r.max_parts = (int)(columns < (long long)sms * kWarps ? columns : (long long)sms * kWarps);
   r.ctas = r.max_parts < sms ? r.max_parts : sms;
   r.pref_bytes = ((size_t)(a.B + 1) * 4 + 15) / 16 * 16;
-  r.bytes = r.pref_bytes + (size_t)r.max_parts * 2 * 8 * r.NB * (a.D + 2) * 4;
+  r.bytes = (r.pref_bytes + (size_t)r.max_parts * 2 * 8 * r.NB * (a.D + 2) * 4 + 15) / 16 * 16;
   return r;
 }
 
+// The sequences of few rows (NB 0: none) and of many of one launch, and the merge.
 template <int D, int NB>
-int rows_launch(PagedParams p, const RowsPlan& r, void* scratch, cudaStream_t stream) {
-  p.pref = static_cast<int*>(scratch);
-  p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + r.pref_bytes);
-  p.max_parts = r.max_parts;
-  static bool configured[64] = {false};
-  int dev = 0;
-  L3CI_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    L3CI_CUDA_TRY(cudaFuncSetAttribute(paged_rows_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem(kPagedMaxSeqs)));
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
-  L3CI_LAUNCH("paged_rows_kernel", paged_rows_kernel<D, NB>, dim3((unsigned)r.ctas), dim3(kThreads), rows_smem(p.a.B), stream, p);
-  // about four parts a group of lanes, but a unit's parts at once where there are few units
-  const long long units = (long long)p.a.B * p.a.Hkv, each = r.max_parts / units;
-  constexpr int kSets = kMergeThreads / (D / 4);
+int launch(PagedParams p, const RowsPlan& r, bool many, void* scratch, cudaStream_t stream) {
   int groups = 1;
-  while (groups < kSets && each > 4 * groups) groups *= 2;
-  const long long items = units * r.row_slots, per_cta = kSets / groups;
-  L3CI_LAUNCH("paged_merge_kernel", paged_merge_kernel<D, NB>, dim3((unsigned)((items + per_cta - 1) / per_cta)), dim3(kMergeThreads), 0, stream, p, groups, r.row_slots);
+  long long rows_ctas = 0;
+  ChunkParams cp = {};
+  if constexpr (NB > 0) {
+    p.min_rows = 1;
+    p.max_rows = kFewRows;
+    p.pref = static_cast<int*>(scratch);
+    p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + r.pref_bytes);
+    p.max_parts = r.max_parts;
+    static bool configured[64] = {false};
+    int dev = 0;
+    L3CI_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+      L3CI_CUDA_TRY(cudaFuncSetAttribute(paged_rows_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem(kPagedMaxSeqs)));
+      if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    L3CI_LAUNCH("paged_rows_kernel", paged_rows_kernel<D, NB>, dim3((unsigned)r.ctas), dim3(kThreads), rows_smem(p.a.B), stream, p);
+    // about four parts a group of lanes, but a unit's parts at once where there are few units
+    const long long units = (long long)p.a.B * p.a.Hkv, each = r.max_parts / units;
+    constexpr int kSets = kMergeThreads / (D / 4);
+    while (groups < kSets && each > 4 * groups) groups *= 2;
+    rows_ctas = (units * r.row_slots + kSets / groups - 1) / (kSets / groups);
+  }
+  long long chunk_ctas = 0;
+  if (many) {
+    PagedParams c = p;
+    c.min_rows = kFewRows + 1;
+    c.max_rows = INT32_MAX;
+    // (its own part of the scratch: where both kernels run, the second does not wait for the first)
+    if (int st = paged_chunks_launch(c, static_cast<uint8_t*>(scratch) + (NB > 0 ? r.bytes : 0), NB > 0, stream, &cp)) return st;
+    chunk_ctas = (long long)(cp.p.max_parts - 1) * kShares<D>;
+  }
+  if (rows_ctas + chunk_ctas > 0)
+    L3CI_LAUNCH("paged_merge_kernel", paged_merge_kernel<D, NB>, dim3((unsigned)(rows_ctas + chunk_ctas)), dim3(kMergeThreads), 0, stream, p, groups, r.row_slots, (int)rows_ctas, cp);
   return L3CI_OK;
 }
 
@@ -609,11 +703,7 @@ size_t scratch_of(PagedParams p) {
     p.max_rows = kFewRows;
     bytes = rows_plan(p).bytes;
   }
-  if (many) {
-    const size_t more = paged_chunks_scratch_bytes(p);
-    if (more > bytes) bytes = more;
-  }
-  return bytes;
+  return bytes + (many ? paged_chunks_scratch_bytes(p) : 0);
 }
 
 }  // namespace
@@ -649,19 +739,13 @@ extern "C" int l3ci_paged_attention(const l3ci_paged_attention_args* a) {
       p.a.out = static_cast<__nv_bfloat16*>(a->out) + b0 * a->o_sb;
       p.a.rows = (long long)p.a.B * p.a.T;
     }
-    if (few) {
-      p.min_rows = 1;
-      p.max_rows = kFewRows;
-      const RowsPlan r = rows_plan(p);
-      const int st = a->D == 64 ? (r.NB == 1 ? rows_launch<64, 1>(p, r, a->scratch, stream) : rows_launch<64, 2>(p, r, a->scratch, stream))
-                                : (r.NB == 1 ? rows_launch<128, 1>(p, r, a->scratch, stream) : rows_launch<128, 2>(p, r, a->scratch, stream));
-      if (st) return st;
-    }
-    if (many) {
-      p.min_rows = kFewRows + 1;
-      p.max_rows = INT32_MAX;
-      if (int st = paged_chunks_launch(p, a->scratch, stream)) return st;
-    }
+    p.max_rows = kFewRows;
+    const RowsPlan r = few ? rows_plan(p) : RowsPlan{};
+    auto go = [&](auto d) {
+      constexpr int D = decltype(d)::value;
+      return r.NB == 0 ? launch<D, 0>(p, r, many, a->scratch, stream) : r.NB == 1 ? launch<D, 1>(p, r, many, a->scratch, stream) : launch<D, 2>(p, r, many, a->scratch, stream);
+    };
+    if (int st = a->D == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{})) return st;
   }
   return L3CI_OK;
 }

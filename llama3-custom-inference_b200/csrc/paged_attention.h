@@ -46,8 +46,30 @@ __device__ __forceinline__ long long paged_row0(const PagedParams& p, int b, lon
 }
 #endif
 
-// paged_attention_tc.cu
+// Chunks of many rows (paged_attention_tc.cu): a unit is two tiles of 128 query rows of a KV head.
+constexpr int kChunkRows = 128;
+// The unit that part g of the deal begins in the middle of, written by its CTA for the merge; parts 0: none, or its first cut is another part's.
+struct ChunkCut {
+  int b, h, m, first, last, parts;
+  int pad[2];
+};
+struct ChunkParams {
+  PagedParams p;
+  ChunkCut* cuts;
+  int tile_tokens;   // tokens of a tile of query rows: 128 / R
+  int box;           // tokens of a copy
+  int follows;       // launched behind paged_rows_kernel of the same call, which has waited for the kernels before
+};
+// Floats of a part: o[D / 4][256 rows][4], m[256], l[256].
+constexpr long long chunk_part_floats(int D) { return 2 * kChunkRows * (D + 2); }
+#if defined(__CUDACC__)
+template <int D>
+__device__ __forceinline__ float* chunk_part_of(const PagedParams& p, int part, bool begins) {
+  return p.records + (2 * part + (begins ? 1 : 0)) * chunk_part_floats(D);
+}
+#endif
+
 size_t paged_chunks_scratch_bytes(const PagedParams& p);
-int paged_chunks_launch(const PagedParams& p, void* scratch, cudaStream_t stream);
+int paged_chunks_launch(const PagedParams& p, void* scratch, bool follows, cudaStream_t stream, ChunkParams* launched);
 
 }  // namespace l3ci

@@ -8,7 +8,7 @@
 //   * keys come page by page: a tile of 128 keys is filled by copies of as many tokens as lie together in every page (a power of two from 16),
 //     each lane of the producer with its own page;
 //   * tiles of keys of all units are dealt in equal runs to the CTAs, by lengths that the device alone knows; a unit that a run's end cuts goes to
-//     scratch as maximum, sum and fp32 products, and paged_chunk_merge_kernel puts the parts together;
+//     scratch as maximum, sum and fp32 products, and paged_merge_kernel puts the parts together;
 //   * what lies behind a sequence's end in its last page, and values that some rows of a tile must not see, may be no numbers, and a
 //     weight of 0 does not stop them: two guard warps look through V tiles at the diagonal and the end, under the first product and the softmax
 //     of the same tile, take such values out, and the output group adds them to the rows that see them.
@@ -29,7 +29,7 @@
 namespace l3ci {
 namespace {
 
-constexpr int kRows = 128;     // query rows of a tile (M of the products)
+constexpr int kRows = kChunkRows;   // query rows of a tile (M of the products)
 constexpr int kKeys = 128;     // keys of a tile
 constexpr int kStages = 2;
 constexpr int kSoftmaxWarps = 8;
@@ -39,32 +39,9 @@ constexpr int kRegsLow = 56, kRegsHigh = 192, kRegsOut = 72;   // of the produce
 static_assert(4 * kRegsLow + kSoftmaxWarps * kRegsHigh + 4 * kRegsOut <= 16 * 128, "register re-deal");
 constexpr uint32_t kTmemCols = 512;                            // S_0, S_1 (128 columns each), O_0, O_1 (D columns each)
 constexpr int kSegments = 8;   // of the ring (the guards are at most three ahead of the output: one-tile segments, two in the ring of V, one on its way out)
-constexpr int kMergeThreads = 256;
 // Columns that a tile counts in the deal, and a unit beside its tiles: its start and its end.
 constexpr int kTileCost = 2;
-constexpr int unit_cost(int D) { return D == 128 ? 2 : 1; }
-constexpr int kMergeItems = 4;                                 // float4 a thread merges
-
-// The unit that part g of the deal begins in the middle of, written by its CTA for the merge; parts 0: none, or its first cut is another part's.
-struct Cut {
-  int b, h, m, first, last, parts;
-  int pad[2];
-};
-
-struct ChunkParams {
-  PagedParams p;
-  Cut* cuts;
-  int tile_tokens;   // tokens of a tile of query rows: 128 / R
-  int box;           // tokens of a copy
-};
-
-// Floats of a part: o[D / 4][256 rows][4], m[256], l[256].
-template <int D>
-__host__ __device__ constexpr long long part_floats() { return 2 * kRows * (D + 2); }
-template <int D>
-__device__ __forceinline__ float* part_of(const PagedParams& p, int part, bool begins) {
-  return p.records + (2 * part + (begins ? 1 : 0)) * part_floats<D>();
-}
+constexpr int unit_cost(int D) { return D == 128 ? 3 : 1; }
 
 // Keys that the tokens of block m (2 * tile_tokens tokens) of a sequence see, in tiles; at least one.
 __device__ __forceinline__ int unit_tiles(const PagedSeq& s, int m, int block) {
@@ -127,7 +104,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     tmem_alloc(smem_u32(tmem_slot), kTmemCols);
     tmem_relinquish();
   }
-  pdl_wait();
+  if (!cp.follows) pdl_wait();
   // ---- columns of the deal before every sequence ----
   constexpr int kUnitCost = unit_cost(D);
   const int block = 2 * cp.tile_tokens;
@@ -230,7 +207,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       on = u.first + kUnitCost < end && tiles_from(u, end) > tiles_from(u, begin);
     }
     if (lane == 0) {      // what the merge has to know of a unit that this run begins in the middle of
-      Cut cut = {};
+      ChunkCut cut = {};
       if (on && u.first + kUnitCost < begin) {
         cut.first = fd_cta_of(u.first + kUnitCost, total, parts);
         if (cut.first == part - 1) {
@@ -574,7 +551,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const int t0 = s.t0 + e * cp.tile_tokens, tokens = min(cp.tile_tokens, s.n - t0);   // tokens of the tile
         const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kSegments) != 0;
         const float inv = lm.x == 0.f ? 0.f : 1.f / lm.x;
-        float* rec = part_of<D>(p, part, j0 == 0);
+        float* rec = chunk_part_of<D>(p, part, j0 == 0);
         const uint32_t to = t_o[e] + lane_addr;
         if (__builtin_expect(taken, 0)) {
           // values that the guards took out, for the rows that see them: from the cache, key by key, into O_e (a call with such values is lost anyway)
@@ -660,6 +637,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
   }
   if (!ok && lane == 0 && a.status) atomicExch(a.status, (int)L3CI_ERR_DEVICE_WAIT);
+  if (cp.follows) pdl_wait();              // (the merge behind counts on both kernels)
   __syncwarp();
   tc_fence_before();
   // a wait ran out: the copies still under way land before the shared memory is given back (or their own waits run out too)
@@ -672,70 +650,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
-}
-
-// Puts the parts of a cut unit together: blockIdx.x the part that it is cut at first, blockIdx.y a share of its rows and columns.
-template <int D>
-__global__ void __launch_bounds__(kMergeThreads) paged_chunk_merge_kernel(const ChunkParams cp) {
-  const PagedParams& p = cp.p;
-  const l3ci_paged_attention_args& a = p.a;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int4 c0 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + blockIdx.x + 1)), c1 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + blockIdx.x + 1) + 1);
-  const int b = c0.x, h = c0.y, m = c0.z, first = c0.w, parts = c1.y;
-  if (parts < 2) return;
-  const PagedSeq s = paged_seq(p, b);
-  const int t_unit = m * 2 * cp.tile_tokens;
-  const long long row0 = paged_row0(p, b, a.o_sb, a.o_st);
-  // neighbouring lanes: 8 rows of 4 vectors each (runs of 128 bytes of a part, of 32 bytes of the result)
-  constexpr int kPerRow = D / 4;
-#pragma unroll 1
-  for (int i = 0; i < kMergeItems; ++i) {
-    const int item = (blockIdx.y * kMergeItems + i) * kMergeThreads + threadIdx.x;
-    const int in8 = item & 31, rest = item >> 5;
-    const int vec = (rest % (kPerRow / 4)) * 4 + (in8 >> 3), row = rest / (kPerRow / 4) * 8 + (in8 & 7);   // row: 0 .. 255
-    const int e = row / kRows, t = (row % kRows) / p.R, token = t_unit + e * cp.tile_tokens + t;
-    if (t >= cp.tile_tokens || token >= s.n) continue;
-    float mx = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kAtOnce = 4;
-    for (int p0 = 0; p0 < parts; p0 += kAtOnce) {
-      float mv[kAtOnce], lv[kAtOnce];
-      float4 ov[kAtOnce];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        mv[k] = -INFINITY;
-        lv[k] = 0.f;
-        ov[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p0 + k < parts) {
-          const float* rec = part_of<D>(p, first + p0 + k, p0 + k == 0);
-          ov[k] = __ldcg(reinterpret_cast<const float4*>(rec) + vec * (2 * kRows) + row);
-          mv[k] = __ldcg(rec + 2 * kRows * D + row);
-          lv[k] = __ldcg(rec + 2 * kRows * (D + 1) + row);
-        }
-      }
-      float mn = mx;
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, mv[k]);
-      const float mu = mn == -INFINITY ? 0.f : mn, w0 = fast_exp2(mx - mu);
-      l *= w0;
-      acc.x *= w0; acc.y *= w0; acc.z *= w0; acc.w *= w0;
-      mx = mn;
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        if (p0 + k >= parts) break;
-        const float w = fast_exp2(mv[k] - mu);
-        l = fmaf(lv[k], w, l);
-        acc.x = fmaf(ov[k].x, w, acc.x);
-        acc.y = fmaf(ov[k].y, w, acc.y);
-        acc.z = fmaf(ov[k].z, w, acc.z);
-        acc.w = fmaf(ov[k].w, w, acc.w);
-      }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 + token * a.o_st + (long long)(h * p.R + row % kRows - t * p.R) * a.o_sh;
-    *reinterpret_cast<uint2*>(out + vec * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  }
 }
 
 // ---- host ----
@@ -791,12 +705,7 @@ int chunk_launch(const ChunkParams& cp, cudaStream_t stream) {
     L3CI_CUDA_TRY(cudaFuncSetAttribute(paged_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem(D, kPagedMaxSeqs)));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int parts = cp.p.max_parts;
-  L3CI_LAUNCH("paged_chunk_kernel", paged_chunk_kernel<D>, dim3((unsigned)parts), dim3(kThreads), chunk_smem(D, cp.p.a.B), stream, qmap, kmap, vmap, cp);
-  if (parts > 1) {
-    constexpr int kShares = 2 * kRows * (D / 4) / (kMergeThreads * kMergeItems);
-    L3CI_LAUNCH("paged_chunk_merge_kernel", paged_chunk_merge_kernel<D>, dim3((unsigned)(parts - 1), kShares), dim3(kMergeThreads), 0, stream, cp);
-  }
+  L3CI_LAUNCH("paged_chunk_kernel", paged_chunk_kernel<D>, dim3((unsigned)cp.p.max_parts), dim3(kThreads), chunk_smem(D, cp.p.a.B), stream, qmap, kmap, vmap, cp);
   return L3CI_OK;
 }
 
@@ -804,18 +713,19 @@ int chunk_launch(const ChunkParams& cp, cudaStream_t stream) {
 
 size_t paged_chunks_scratch_bytes(const PagedParams& p) {
   const int parts = chunk_parts(p);
-  return (size_t)parts * (sizeof(Cut) + 2 * 4 * (size_t)(p.a.D == 64 ? part_floats<64>() : part_floats<128>()));
+  return (size_t)parts * (sizeof(ChunkCut) + 2 * 4 * (size_t)(p.a.D == 64 ? chunk_part_floats(64) : chunk_part_floats(128)));
 }
 
-int paged_chunks_launch(const PagedParams& params, void* scratch, cudaStream_t stream) {
-  ChunkParams cp = {};
+int paged_chunks_launch(const PagedParams& params, void* scratch, bool follows, cudaStream_t stream, ChunkParams* launched) {
+  ChunkParams& cp = *launched;
   cp.p = params;
   cp.p.max_parts = chunk_parts(params);
-  cp.cuts = static_cast<Cut*>(scratch);
+  cp.cuts = static_cast<ChunkCut*>(scratch);
   cp.p.records = reinterpret_cast<float*>(cp.cuts + cp.p.max_parts);
   cp.tile_tokens = kRows / params.R;
   const int low = params.a.page_size & -params.a.page_size;    // tokens that lie together in every page: a power of two
   cp.box = low < kKeys ? low : kKeys;
+  cp.follows = follows;
   return params.a.D == 64 ? chunk_launch<64>(cp, stream) : chunk_launch<128>(cp, stream);
 }
 
