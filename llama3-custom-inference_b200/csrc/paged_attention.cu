@@ -34,7 +34,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kSlots = 3;            // tiles in flight per warp
 constexpr int kTileBytes = 8192;     // K then V
 constexpr int kFewRows = 16;
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = kThreads;   // (it counts the columns as the first kernel does)
 
 constexpr size_t rows_smem(int B) { return 1024 + (size_t)kWarps * kSlots * kTileBytes + (size_t)(B + 1) * 4; }
 
@@ -61,6 +61,37 @@ __device__ __forceinline__ float* record_of(const PagedParams& p, int part, bool
   return p.records + (long long)(2 * part + (begins ? 1 : 0)) * (8 * NB * (D + 2));   // o[row][D], m[row], l[row]
 }
 
+// Columns of the deal before every sequence, pref[0 .. B], by all threads of the CTA (kThreads).
+template <int D>
+__device__ __forceinline__ void count_columns(const PagedParams& p, int* pref) {
+  __shared__ int warp_sums[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto columns = [&](int b) {
+    const PagedSeq s = paged_seq(p, b);
+    return s.n > 0 ? p.a.Hkv * fd_tiles(s.len, fd_tile_tokens(D)) : 0;
+  };
+  const int each = (p.a.B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * each, p.a.B), b1 = min(b0 + each, p.a.B);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int c = columns(b);
+    pref[b + 1] = c;
+    mine += c;
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int other = __shfl_up_sync(kFullMask, upto, d);
+    if (lane >= d) upto += other;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  if (threadIdx.x == 0) pref[0] = 0;
+  __syncthreads();
+  int before = upto - mine;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  for (int b = b0; b < b1; ++b) pref[b + 1] = before += pref[b + 1];
+  __syncthreads();
+}
+
 // One warp's walk over the tiles of its run.
 struct Cursor {
   int b, h, tile, tiles;
@@ -75,42 +106,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const PagedPara
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* pref = reinterpret_cast<int*>(smem + kWarps * kSlots * kTileBytes);
-  __shared__ int warp_sums[kWarps];
   const l3ci_paged_attention_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- columns before every sequence ----
-  auto columns = [&](int b) {
-    const PagedSeq s = paged_seq(p, b);
-    return s.n > 0 ? a.Hkv * fd_tiles(s.len, kTile) : 0;
-  };
-  {
-    const int each = (a.B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * each, a.B), b1 = min(b0 + each, a.B);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += columns(b);
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int other = __shfl_up_sync(kFullMask, upto, d);
-      if (lane >= d) upto += other;
-    }
-    if (lane == 31) warp_sums[warp] = upto;
-    __syncthreads();
-    int before = upto - mine;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    for (int b = b0; b < b1; ++b) {
-      pref[b] = before;
-      before += columns(b);
-    }
-    if (b1 == a.B && b0 < b1) pref[a.B] = before;
-    __syncthreads();
-  }
+  count_columns<D>(p, pref);
   const int total = pref[a.B];
-  if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b <= a.B; b += kThreads) p.pref[b] = pref[b];
   const int parts = parts_of(total, p.max_parts), part = warp * (int)gridDim.x + (int)blockIdx.x;   // (few parts: one per SM)
   if (part >= parts) return;
   const int begin = fd_range_begin(part, total, parts), end = fd_range_begin(part + 1, total, parts);
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const PagedPara
 // Merges the parts of the units of few rows that were cut.  D / 4 lanes per query row and group of parts, `groups` (a power of two) groups of parts
 // per row.
 template <int D, int NB>
-__device__ __forceinline__ void merge_rows(const PagedParams& p, int groups, int row_slots, int cta) {
+__device__ __forceinline__ void merge_rows(const PagedParams& p, const int* pref, int groups, int row_slots, int cta) {
   constexpr int kTile = fd_tile_tokens(D), kLanes = D / 4, kSets = kMergeThreads / kLanes;
   __shared__ float4 sums[kSets][kLanes];
   __shared__ float2 stats[kSets];
@@ -433,8 +436,8 @@ __device__ __forceinline__ void merge_rows(const PagedParams& p, int groups, int
   live = live && row < s.n * p.R;
   int first = 0, last = 0, parts = 1, total = 0;
   if (live) {
-    const int tiles = fd_tiles(s.len, kTile), begin = __ldcg(p.pref + b) + h * tiles;
-    total = __ldcg(p.pref + a.B);
+    const int tiles = fd_tiles(s.len, kTile), begin = pref[b] + h * tiles;
+    total = pref[a.B];
     parts = parts_of(total, p.max_parts);
     first = fd_cta_of(begin, total, parts);
     last = fd_cta_of(begin + tiles - 1, total, parts);
@@ -575,10 +578,14 @@ __device__ __forceinline__ void merge_chunk(const ChunkParams& cp, int cta) {
 // NB 0: no sequences of few rows.  The first rows_ctas CTAs are theirs.
 template <int D, int NB>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedParams p, int groups, int row_slots, int rows_ctas, const ChunkParams cp) {
+  extern __shared__ int merge_pref[];
+  // (the lengths were complete before the first kernel of the call let the next one start)
+  const bool rows = NB > 0 && (int)blockIdx.x < rows_ctas;
+  if (rows) count_columns<D>(p, merge_pref);
   pdl_wait();
   pdl_launch_dependents();
   if constexpr (NB > 0)
-    if ((int)blockIdx.x < rows_ctas) return merge_rows<D, NB>(p, groups, row_slots, blockIdx.x);
+    if (rows) return merge_rows<D, NB>(p, merge_pref, groups, row_slots, blockIdx.x);
   merge_chunk<D>(cp, blockIdx.x - rows_ctas);
 }
 
@@ -611,7 +618,7 @@ namespace {
 // How a launch over sequences of few rows is laid out.
 struct RowsPlan {
   int NB, ctas, max_parts, row_slots;
-  size_t pref_bytes, bytes;      // of scratch
+  size_t bytes;                  // of scratch
 };
 
 RowsPlan rows_plan(const PagedParams& p) {
@@ -624,8 +631,7 @@ RowsPlan rows_plan(const PagedParams& p) {
   const long long columns = (long long)a.B * a.Hkv * fd_tiles(p.cap, fd_tile_tokens(a.D));
   r.max_parts = (int)(columns < (long long)sms * kWarps ? columns : (long long)sms * kWarps);
   r.ctas = r.max_parts < sms ? r.max_parts : sms;
-  r.pref_bytes = ((size_t)(a.B + 1) * 4 + 15) / 16 * 16;
-  r.bytes = (r.pref_bytes + (size_t)r.max_parts * 2 * 8 * r.NB * (a.D + 2) * 4 + 15) / 16 * 16;
+  r.bytes = (size_t)r.max_parts * 2 * 8 * r.NB * (a.D + 2) * 4;
   return r;
 }
 
@@ -638,8 +644,7 @@ int launch(PagedParams p, const RowsPlan& r, bool many, void* scratch, cudaStrea
   if constexpr (NB > 0) {
     p.min_rows = 1;
     p.max_rows = kFewRows;
-    p.pref = static_cast<int*>(scratch);
-    p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + r.pref_bytes);
+    p.records = static_cast<float*>(scratch);
     p.max_parts = r.max_parts;
     static bool configured[64] = {false};
     int dev = 0;
@@ -649,10 +654,10 @@ int launch(PagedParams p, const RowsPlan& r, bool many, void* scratch, cudaStrea
       if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     L3CI_LAUNCH("paged_rows_kernel", paged_rows_kernel<D, NB>, dim3((unsigned)r.ctas), dim3(kThreads), rows_smem(p.a.B), stream, p);
-    // about four parts a group of lanes, but a unit's parts at once where there are few units
+    // up to eight parts a group of lanes (four: twice the CTAs, two waves of them, 16 sequences of 8 KV heads of 8 query heads 8.2 us instead of 5.2)
     const long long units = (long long)p.a.B * p.a.Hkv, each = r.max_parts / units;
     constexpr int kSets = kMergeThreads / (D / 4);
-    while (groups < kSets && each > 4 * groups) groups *= 2;
+    while (groups < kSets && each > 8 * groups) groups *= 2;
     rows_ctas = (units * r.row_slots + kSets / groups - 1) / (kSets / groups);
   }
   long long chunk_ctas = 0;
@@ -665,7 +670,7 @@ int launch(PagedParams p, const RowsPlan& r, bool many, void* scratch, cudaStrea
     chunk_ctas = (long long)(cp.p.max_parts - 1) * kShares<D>;
   }
   if (rows_ctas + chunk_ctas > 0)
-    L3CI_LAUNCH("paged_merge_kernel", paged_merge_kernel<D, NB>, dim3((unsigned)(rows_ctas + chunk_ctas)), dim3(kMergeThreads), 0, stream, p, groups, r.row_slots, (int)rows_ctas, cp);
+    L3CI_LAUNCH("paged_merge_kernel", paged_merge_kernel<D, NB>, dim3((unsigned)(rows_ctas + chunk_ctas)), dim3(kMergeThreads), NB > 0 ? (size_t)(p.a.B + 1) * 4 : 0, stream, p, groups, r.row_slots, (int)rows_ctas, cp);
   return L3CI_OK;
 }
 

@@ -18,7 +18,6 @@ struct PagedParams {
   int min_rows, max_rows;   // query rows (tokens x R) of the sequences that the launch takes
   int max_parts;       // CTAs or warps that work is dealt to
   float scale_log2e;
-  int* pref;           // scratch: columns before each sequence [B + 1]
   float* records;      // scratch: partial results
 };
 

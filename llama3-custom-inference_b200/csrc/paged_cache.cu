@@ -12,17 +12,62 @@
 #include "host_common.h"
 #include "ptx_sm100.cuh"
 #include "rotate.cuh"
+#include "tcgen05.cuh"
 #include "warp_reduce.cuh"
 
 namespace l3ci {
 namespace {
 
 constexpr int kBlock = 128;
-constexpr int kBatch = 4;   // 16-byte loads a thread has in flight
+constexpr int kBatch = 4;   // 16-byte loads of queries a thread has in flight
+
+typedef unsigned long long f2;   // two floats
+
+// What a vector's four pairs are multiplied with: (x, y) -> x (c w_x, s w_x) + y (-s w_y, c w_y), the norm's weights in the rotation.
+struct Turn {
+  f2 x[4], y[4];
+};
+__device__ __forceinline__ Turn turn_of(const float4& f0, const float4& f1, const uint4& weights) {
+  float w[8];
+  unpack8(weights, w);
+  const float c[4] = {f0.x, f0.z, f1.x, f1.z}, s[4] = {f0.y, f0.w, f1.y, f1.w};
+  Turn t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t.x[i] = f2_packf(c[i] * w[2 * i], s[i] * w[2 * i]);
+    t.y[i] = f2_packf(-s[i] * w[2 * i + 1], c[i] * w[2 * i + 1]);
+  }
+  return t;
+}
+// A head's vector normed and rotated; LANES lanes hold the head.
+template <int LANES>
+__device__ __forceinline__ uint4 norm_rotate8(const uint4& v, const Turn& t, float over_d, float eps) {
+  float a[8];
+  unpack8(v, a);
+  f2 ss = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f2 p = f2_packf(a[2 * i], a[2 * i + 1]);
+    ss = f2_fma(p, p, ss);
+  }
+  float s0, s1;
+  f2_unpack(ss, s0, s1);
+  const float rs = rsqrtf(fmaf(group_sum<LANES>(s0 + s1), over_d, eps));
+  const f2 rs2 = f2_packf(rs, rs);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f2 turned = f2_fma(f2_packf(a[2 * i], a[2 * i]), t.x[i], f2_mul(f2_packf(a[2 * i + 1], a[2 * i + 1]), t.y[i]));
+    float x, y;
+    f2_unpack(f2_mul(turned, rs2), x, y);
+    o[i] = pack_bf16x2(x, y);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
 
 // LANES: lanes that hold a head, a power of two of at least D / 8 (those beyond it have nothing).
 template <int LANES, bool NORM>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, NORM ? 7 : 9)
 rot_embed_paged_kv_cache_kernel(const l3ci_paged_rope_args p) {
   __shared__ int found;
   if (threadIdx.x == 0) found = -1;
@@ -30,20 +75,22 @@ rot_embed_paged_kv_cache_kernel(const l3ci_paged_rope_args p) {
   const long long row = blockIdx.x;
   int b = p.starts ? 0 : (int)(row / p.T);
   long long t = p.starts ? 0 : row % p.T;
-  const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(p.qkv) + (p.starts ? row * p.qkv_st : b * p.qkv_sb + t * p.qkv_st);
   const int vecs = p.D / kVecElems, vec = threadIdx.x % LANES, head0 = threadIdx.x / LANES;
   constexpr int kHeads = kBlock / LANES;                       // heads the CTA takes at a time
-  const int heads = p.Hq + 2 * p.Hkv;
   const bool mine = vec < vecs;
-  uint4 v[kBatch];
-  auto load = [&](int h0) {
+  const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(p.qkv) + (p.starts ? row * p.qkv_st : b * p.qkv_sb + t * p.qkv_st) + vec * kVecElems;
+  const __nv_bfloat16 *in_k = in + p.Hq * p.D, *in_v = in_k + p.Hkv * p.D;
+  auto load = [&](const __nv_bfloat16* from, int h, int heads) { return mine && h < heads ? ld_stream16(from + h * p.D) : make_uint4(0, 0, 0, 0); };
+  uint4 q[kBatch], k, v;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int h = h0 + u * kHeads;
-      v[u] = mine && h < heads ? ld_stream16(in + h * p.D + vec * kVecElems) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  load(head0);
+  for (int u = 0; u < kBatch; ++u) q[u] = load(in, head0 + u * kHeads, p.Hq);
+  k = load(in_k, head0, p.Hkv);
+  v = load(in_v, head0, p.Hkv);
+  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
+  if (NORM && mine) {
+    wq = __ldg(static_cast<const uint4*>(p.q_norm) + vec);
+    wk = __ldg(static_cast<const uint4*>(p.k_norm) + vec);
+  }
   if (p.starts) {
     __syncthreads();                                           // (found is set)
     for (int i = threadIdx.x; i < p.B; i += kBlock)
@@ -60,52 +107,47 @@ rot_embed_paged_kv_cache_kernel(const l3ci_paged_rope_args p) {
   const int page = __ldg(p.page_table + b * p.table_st + slot);
   if (page < 0 || page >= p.pages) return;
   float4 f0 = make_float4(0, 0, 0, 0), f1 = f0;
-  float wq[8] = {}, wk[8] = {};
   if (mine) {
     const float* f = p.freq_table + pos * p.D + vec * kVecElems;
     f0 = __ldg(reinterpret_cast<const float4*>(f));
     f1 = __ldg(reinterpret_cast<const float4*>(f) + 1);
-    if (NORM) {
-      unpack8(__ldg(static_cast<const uint4*>(p.q_norm) + vec), wq);
-      unpack8(__ldg(static_cast<const uint4*>(p.k_norm) + vec), wk);
-    }
   }
+  const float over_d = 1.f / (float)p.D;
+  Turn turn;
+  if (NORM) turn = turn_of(f0, f1, wq);
+  auto turned = [&](const uint4& x) {
+    if constexpr (NORM) return norm_rotate8<LANES>(x, turn, over_d, p.eps);
+    else return rotate8(x, f0, f1);
+  };
   __nv_bfloat16* qo = static_cast<__nv_bfloat16*>(p.q_out) + row * p.q_st + vec * kVecElems;
   const long long at = page * p.cache_sp + (pos - slot * p.page_size) * p.cache_st + vec * kVecElems;
   __nv_bfloat16* ko = static_cast<__nv_bfloat16*>(p.cache_k) + at;
   __nv_bfloat16* vo = static_cast<__nv_bfloat16*>(p.cache_v) + at;
   // (all lanes of a warp take every round: the shuffles of a norm want them)
-  for (int h0 = head0;; h0 += kHeads * kBatch) {
+  for (int h0 = 0; h0 < p.Hq; h0 += kHeads * kBatch) {
+    if (h0 > 0)
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) q[u] = load(in, h0 + head0 + u * kHeads, p.Hq);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int h = h0 + u * kHeads;
-      uint4 r = v[u];
-      if (NORM) {
-        float a[8], o[8];
-        unpack8(r, a);
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], ss);
-        const float rs = rsqrtf(group_sum<LANES>(ss) / (float)p.D + p.eps);
-        const bool is_q = h < p.Hq;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = a[i] * rs * (is_q ? wq[i] : wk[i]);
-        rotate_pair(a[0], a[1], f0.x, f0.y, o[0], o[1]);
-        rotate_pair(a[2], a[3], f0.z, f0.w, o[2], o[3]);
-        rotate_pair(a[4], a[5], f1.x, f1.y, o[4], o[5]);
-        rotate_pair(a[6], a[7], f1.z, f1.w, o[6], o[7]);
-        if (h < p.Hq + p.Hkv) r = pack8(o);
-      } else if (h < p.Hq + p.Hkv) {
-        r = rotate8(r, f0, f1);
-      }
-      if (!mine || h >= heads) continue;
-      if (h < p.Hq) st_stream16(qo + h * p.D, r);
-      // (the cache rows are read again by the attention of the same step: plain stores)
-      else if (h < p.Hq + p.Hkv) *reinterpret_cast<uint4*>(ko + (h - p.Hq) * p.D) = r;
-      else *reinterpret_cast<uint4*>(vo + (h - p.Hq - p.Hkv) * p.D) = r;
+      const int h = h0 + head0 + u * kHeads;
+      const uint4 r = turned(q[u]);
+      if (mine && h < p.Hq) st_stream16(qo + h * p.D, r);
     }
-    if (h0 - head0 + kHeads * kBatch >= heads) break;
-    load(h0 + kHeads * kBatch);
+  }
+  if (NORM) turn = turn_of(f0, f1, wk);
+  // (the cache rows are read again by the attention of the same step: plain stores)
+  for (int h0 = 0; h0 < p.Hkv; h0 += kHeads) {
+    const int h = h0 + head0;
+    if (h0 > 0) {
+      k = load(in_k, h, p.Hkv);
+      v = load(in_v, h, p.Hkv);
+    }
+    const uint4 r = turned(k);
+    if (mine && h < p.Hkv) {
+      *reinterpret_cast<uint4*>(ko + h * p.D) = r;
+      *reinterpret_cast<uint4*>(vo + h * p.D) = v;
+    }
   }
 }
 
