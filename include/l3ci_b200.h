@@ -457,7 +457,8 @@ L3CI_API size_t l3ci_paged_attention_scratch_bytes(const l3ci_paged_attention_ar
  *   out[r] = x[r] w^T + scales[i] (x[r] a[i]^T) b[i]^T,   i = index[r];   i outside [0, adapters): the shared product alone.
  * x bf16 [rows, K] (x_st apart), w bf16 [N, K], a bf16 [adapters, rank, K], b bf16 [adapters, N, rank], all dense, scales fp32
  * [adapters] (null: 1), index int32 [rows] on the device; out bf16 [rows, N] (out_st apart).  Sums in fp32, one rounding at the end.
- * K and N multiples of 8, rank a multiple of 8 up to 128.  scratch: l3ci_adapter_linear_scratch_bytes, as above. */
+ * K and N multiples of 8, rank a multiple of 8 up to 128.  scratch: l3ci_adapter_linear_scratch_bytes, as above.
+ * status: as in l3ci_linear.  No row meets another's adapter, whatever that holds. */
 #define L3CI_ADAPTER_MAX_RANK 128
 typedef struct l3ci_adapter_linear_args {
   const void *x, *w, *a, *b;

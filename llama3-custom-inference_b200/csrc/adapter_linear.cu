@@ -264,5 +264,5 @@ extern "C" int l3ci_adapter_linear(const l3ci_adapter_linear_args* a) {
     if (int st = a->rank <= 8 ? shrink(adapter_shrink_many_kernel<1>, 8) : a->rank <= 16 ? shrink(adapter_shrink_many_kernel<2>, 16) : shrink(adapter_shrink_many_kernel<4>, 32)) return st;
   }
   if (few) return adapter_rows_launch(&l, AdapterRows{z, a->index, b, a->rank, a->adapters});
-  return adapter_many_launch(&l, AdapterMany{z, b, lists, a->rank, a->adapters});
+  return adapter_many_launch(&l, AdapterMany{z, b, lists, a->rank, a->adapters, a->status});
 }

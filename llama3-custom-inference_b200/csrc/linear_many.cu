@@ -364,7 +364,7 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
       }
     }
   }
-  if (!ok && lane == 0) atomicExch(&g_wait_status, (int)L3CI_ERR_DEVICE_WAIT);
+  if (!ok && lane == 0) atomicExch(ADAPT && p.low.status ? p.low.status : &g_wait_status, (int)L3CI_ERR_DEVICE_WAIT);
   __syncwarp();
   tc_fence_before();
   // a wait ran out: the copies still under way land before the shared memory is given back (or their own waits run out too)

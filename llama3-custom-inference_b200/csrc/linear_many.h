@@ -20,6 +20,7 @@ struct AdapterMany {
   const __nv_bfloat16* b;
   const int* lists;
   int rank, adapters;
+  int* status;         // where a wait that ran out is recorded; null: the library's word
 };
 // l3ci_linear_many (one group, no activation) with these parts, one rounding.
 int adapter_many_launch(const l3ci_linear_args* a, const AdapterMany& low);

@@ -12,7 +12,7 @@
 // A token's place comes from the table: a lane holds the place of every 16 tokens of the next 512, asked for one block ahead.
 // The arithmetic of a tile is that of flash_decode_small.cu: S^T = K Q^T and O^T += V^T P^T on mma.sync.m16n8k16, keys on the rows of a
 // tile, query rows on its 8 columns, twice where there are more than 8.  p is rounded to bf16 for the second product (tensor cores take
-// bf16 operands; 2^-9 of each weight on average zero), everything else is fp32.
+// bf16 operands; a weight is off by at most 2^-8 of it), everything else is fp32.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -607,6 +607,8 @@ int check(const l3ci_paged_attention_args* a) {
   // (columns of a sequence, 16 keys of a head each, are counted in 32 bits)
   if (rows > 0x7fffffffLL || a->pages > 0x7fffffffLL || (long long)a->max_pages * a->page_size > (1LL << 30) / (a->Hkv < 16 ? 16 : a->Hkv) * 16)
     return fail(L3CI_ERR_INVALID, "paged_attention: %lld rows, %lld keys a sequence", rows, (long long)a->max_pages * a->page_size);
+  if (paged_chunk_columns(a) > 0x7fffffffLL)
+    return fail(L3CI_ERR_INVALID, "paged_attention: %lld rows over up to %lld keys are too many for one call", rows, (long long)a->max_pages * a->page_size);
   return L3CI_OK;
 }
 

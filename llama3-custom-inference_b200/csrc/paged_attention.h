@@ -68,6 +68,7 @@ __device__ __forceinline__ float* chunk_part_of(const PagedParams& p, int part, 
 }
 #endif
 
+long long paged_chunk_columns(const l3ci_paged_attention_args* a);   // of the deal, at most
 size_t paged_chunks_scratch_bytes(const PagedParams& p);
 int paged_chunks_launch(const PagedParams& p, void* scratch, bool follows, cudaStream_t stream, ChunkParams* launched);
 

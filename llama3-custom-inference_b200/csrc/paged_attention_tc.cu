@@ -660,9 +660,7 @@ size_t chunk_smem(int D, int B) {
 
 int chunk_parts(const PagedParams& p) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
-  // (columns at most: every token's own unit of all the keys that the table can hold)
-  const long long rows = p.a.starts ? p.a.rows : (long long)p.a.B * p.a.T, block = 2 * (kRows / p.R);
-  const long long columns = (rows / block + p.a.B) * p.a.Hkv * (((long long)p.cap + kKeys - 1) / kKeys + 1 + unit_cost(p.a.D));
+  const long long columns = paged_chunk_columns(&p.a);
   return (int)(columns < sms ? columns : sms);
 }
 
@@ -710,6 +708,13 @@ int chunk_launch(const ChunkParams& cp, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// (every block of every sequence a unit over all the keys that the table can hold)
+long long paged_chunk_columns(const l3ci_paged_attention_args* a) {
+  const long long rows = a->starts ? a->rows : (long long)a->B * a->T, block = 2 * (kRows / (a->Hq / a->Hkv));
+  const long long seqs = a->B < kPagedMaxSeqs ? a->B : kPagedMaxSeqs;
+  return (rows / block + seqs) * a->Hkv * (kTileCost * (((long long)a->max_pages * a->page_size + kKeys - 1) / kKeys + 1) + unit_cost(a->D));
+}
 
 size_t paged_chunks_scratch_bytes(const PagedParams& p) {
   const int parts = chunk_parts(p);

@@ -631,6 +631,8 @@ void check_paged(const Tensor& x, const Tensor& cache_k, const Tensor& cache_v, 
   TORCH_CHECK(cache_k.dim() == 4 && cache_k.sizes() == cache_v.sizes() && cache_k.strides() == cache_v.strides(),
               "cache_k and cache_v must be [pages, page_size, n_kv_head, D] with equal layout");
   TORCH_CHECK((cache_k.stride(3) == 1 || cache_k.size(3) == 1) && (cache_k.stride(2) == cache_k.size(3) || cache_k.size(2) == 1), "cache rows must be [n_kv_head, D] contiguous");
+  // (pages and rows that share a place cannot be described to the copy engine, nor written)
+  TORCH_CHECK((cache_k.stride(0) > 0 || cache_k.size(0) <= 1) && (cache_k.stride(1) > 0 || cache_k.size(1) <= 1), "pages and rows of the caches must have places of their own");
   TORCH_CHECK(page_table.is_cuda() && page_table.scalar_type() == torch::kInt32 && page_table.dim() == 2 && (page_table.stride(1) == 1 || page_table.size(1) <= 1),
               "page_table must be an int32 CUDA tensor [B, entries] with contiguous rows");
   const int64_t B = page_table.size(0);
@@ -705,10 +707,17 @@ Tensor paged_attention(Tensor query, Tensor cache_k, Tensor cache_v, Tensor page
   check_paged(query, cache_k, cache_v, page_table, seq_lens, "seq_lens", starts);
   TORCH_CHECK(cache_k.size(3) == query.size(-1), "head size of query and cache differ");
   const c10::cuda::CUDAGuard guard(query.device());
+  auto broadcast = [](const Tensor& t) {
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.stride(d) == 0 && t.size(d) > 1) return true;
+    return false;
+  };
+  if (broadcast(query)) query = query.contiguous();
   Tensor y = out ? *out : torch::empty(query.sizes(), query.options());
   if (out) {
     check_bf16_cuda(y, "out");
     TORCH_CHECK(y.sizes() == query.sizes() && y.get_device() == query.get_device() && (y.stride(-1) == 1 || y.size(-1) == 1), "out must be shaped like query, on its device");
+    TORCH_CHECK(!broadcast(y), "the rows of out must have places of their own");
   }
   l3ci_paged_attention_args a{};
   a.q = query.data_ptr(); a.cache_k = cache_k.data_ptr(); a.cache_v = cache_v.data_ptr(); a.out = y.data_ptr();

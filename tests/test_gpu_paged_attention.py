@@ -65,6 +65,25 @@ def test_many_short_sequences_beside_one_long(ext, device):
     check(run(ext, case), case)
 
 
+def test_more_sequences_than_a_launch_takes(ext, device):
+    # 2048 sequences a launch: one token each, and packed rows with a chunk on either side of the border
+    totals = [1 + 5 * i % 37 for i in range(2500)]
+    case = attention_case([1] * 2500, totals, 4, 2, 64, 16, device, seed=1, packed=False)
+    check(run(ext, case), case)
+    new = [1] * 2040 + [20, 3, 0, 70, 1, 1, 9, 2, 33, 1] + [1] * 30
+    case = attention_case(new, [n + i % 41 for i, n in enumerate(new)], 4, 2, 64, 16, device, seed=2)
+    check(run(ext, case), case)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_queries_that_are_broadcast(ext, device, new):
+    case = attention_case([new] * 3, [100, 200, 300], 8, 2, 64, 16, device, seed=new, packed=False)
+    one = case.q[:1, :, :1]
+    got = ext.paged_attention(one.expand(3, new, 8, 64), case.k, case.v, case.table, case.seq_lens)
+    case.rows = one.expand(3, new, 8, 64).reshape(-1, 8, 64).contiguous()
+    check(got, case)
+
+
 def test_lengths_that_leave_tokens_without_keys(ext, device):
     # fewer tokens cached than are new: the first ones see nothing; a length of zero; one beyond the table's row is clamped
     case = attention_case([5, 40, 3, 1, 300], [64, 64, 64, 64, 320], 8, 2, 128, 16, device, seed=9)
@@ -227,7 +246,8 @@ def test_refusals(ext, device):
         (dict(page_table=table.long()), "int32"), (dict(page_table=table.t()), "contiguous rows"), (dict(seq_lens=lens.long()), "int32"),
         (dict(seq_lens=lens[:1]), r"\[B\]"), (dict(starts=torch.zeros(2, dtype=torch.int32, device=device), query=q[:, 0]), r"\[B \+ 1\]"),
         (dict(out=torch.zeros(2, 1, 4, 32, dtype=BF16, device=device)), "shaped like query"),
-        (dict(out=torch.zeros(2, 1, 4, 64, device=device)), "bfloat16"),
+        (dict(out=torch.zeros(2, 1, 4, 64, device=device)), "bfloat16"), (dict(out=q[:1].clone().expand(2, 1, 4, 64)), "places of their own"),
+        (dict(cache_k=k[:1].expand(4, 16, 2, 64), cache_v=k[:1].expand(4, 16, 2, 64)), "places of their own"),
     ]
     for change, words in bad:
         with pytest.raises(RuntimeError, match=words):

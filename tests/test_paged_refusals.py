@@ -32,7 +32,7 @@ def test_paged_attention(capi):
     go = lambda **kw: call(capi, "l3ci_paged_attention", capi.PagedAttentionArgs, good, **kw)  # noqa: E731
     for bad in (dict(q=None), dict(cache_k=None), dict(cache_v=None), dict(out=None), dict(page_table=None), dict(seq_lens=None), dict(B=-1), dict(T=-1), dict(Hq=0),
                 dict(Hkv=0), dict(page_size=0), dict(max_pages=-1), dict(pages=-1), dict(starts=FAKE, rows=-1), dict(max_pages=2 ** 30), dict(pages=2 ** 31),
-                dict(starts=FAKE, rows=2 ** 31)):
+                dict(starts=FAKE, rows=2 ** 31), dict(starts=FAKE, rows=2 ** 22, max_pages=2 ** 18)):
         assert go(**bad) == capi.ERR_INVALID, bad
     for bad in (dict(D=96), dict(Hq=5), dict(Hq=34), dict(page_size=24), dict(page_size=8)):
         assert go(**bad) == capi.ERR_UNSUPPORTED, bad
