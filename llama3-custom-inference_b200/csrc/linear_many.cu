@@ -223,7 +223,7 @@ linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
   } else if (warp == 1 && rank == 0) {
     // ---- MMA issue, for both: all lanes run the code, one elected lane predicates the instructions ----
     constexpr uint32_t idesc = instr_desc(2 * kHalf, kCols, false);
-    const uint32_t elected = lane == 0 ? 1u : 0u;
+    const uint32_t elected = elect_one();
     int s = 0, round = 0, filled = 0;
     uint32_t parity = 0;
     for (long long tile = pair; tile < p.tiles && ok; tile += pairs, ++round) {

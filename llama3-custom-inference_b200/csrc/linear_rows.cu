@@ -288,7 +288,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     // ---- MMA issue: all lanes run the code, one elected lane predicates the instructions ----
     if (!ADAPT) pdl_wait();              // (the bounds of the waits below count from here, not through the kernels before)
     constexpr uint32_t idesc = instr_desc(kTile, Sh::kCols, false);
-    const uint32_t elected = lane == 0 ? 1u : 0u;
+    const uint32_t elected = elect_one();
     int s = 0, round = 0;
     uint32_t parity = 0;
     for (int tile = first; tile < p.tiles && ok; tile += stride, ++round) {

@@ -13,6 +13,8 @@
 // The arithmetic of a tile is that of flash_decode_small.cu: S^T = K Q^T and O^T += V^T P^T on mma.sync.m16n8k16, keys on the rows of a
 // tile, query rows on its 8 columns, twice where there are more than 8.  p is rounded to bf16 for the second product (tensor cores take
 // bf16 operands; a weight is off by at most 2^-8 of it), everything else is fp32.
+// Measured on a B200: 16 sequences of 3500 to 8000 keys, 64 query on 8 KV heads of 128, pages of 16, 384 MB: 63.4 us, 6.05 TB/s, and 5.2 for the
+// merge (eight parts at a time; one after the other 8); a sequence of 131072 keys, 32 on 8 heads, 537 MB: 83.6 us, 6.4 TB/s, and 7.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -607,7 +609,7 @@ int check(const l3ci_paged_attention_args* a) {
   // (columns of a sequence, 16 keys of a head each, are counted in 32 bits)
   if (rows > 0x7fffffffLL || a->pages > 0x7fffffffLL || (long long)a->max_pages * a->page_size > (1LL << 30) / (a->Hkv < 16 ? 16 : a->Hkv) * 16)
     return fail(L3CI_ERR_INVALID, "paged_attention: %lld rows, %lld keys a sequence", rows, (long long)a->max_pages * a->page_size);
-  if (paged_chunk_columns(a) > 0x7fffffffLL)
+  if ((a->starts ? a->rows : a->T) * (a->Hq / a->Hkv) > kFewRows && paged_chunk_columns(a) > 0x7fffffffLL)
     return fail(L3CI_ERR_INVALID, "paged_attention: %lld rows over up to %lld keys are too many for one call", rows, (long long)a->max_pages * a->page_size);
   return L3CI_OK;
 }

@@ -12,6 +12,12 @@
 //   * what lies behind a sequence's end in its last page, and values that some rows of a tile must not see, may be no numbers, and a
 //     weight of 0 does not stop them: two guard warps look through V tiles at the diagonal and the end, under the first product and the softmax
 //     of the same tile, take such values out, and the output group adds them to the rows that see them.
+// Measured on a B200: 2 x 512 tokens of 16500 keys, 32 query on 8 KV heads of 128, any page size 243 us, 1120 TFLOP/s, heads of 64 227, 600; a prompt of
+// 4096 tokens, heads of 128 155 us, 890, of 64 130, 530 (a head of 64 has half the products to the same exponentials).  A tile of keys takes
+// 3650 cycles (heads of 128), of which a warp's softmax is 2030 (its exponentials alone 1450 for the 1024 that they cannot do without) and
+// the wait for the products between 1240; the tensor cores need 2050 and the exponentials of both groups as much.  For heads of 64 the weights
+// in a place of their own, so that the next scores come under the exponentials: both groups then take theirs at once, 234 us instead of 227.
+// Scores read from tensor memory twice by loops of 32 keys instead of once: 3 to 10 % slower.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -293,10 +299,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
-    // ---- MMA issue: all lanes run the code, one elected lane predicates the instructions ----
+    // ---- MMA issue: all lanes run the code, one issues the instructions; what all lanes agree on comes out of a shuffle, so that the compiler knows it too
+    // (elect_one).  With `lane == 0` and plain registers this warp bounded the kernel: 2 x 512 tokens of 16500 keys of 32 heads of 128 took 283 us
+    // instead of 243 (960 and 1120 TFLOP/s), a prompt of 4096 tokens of heads of 64 142 instead of 130 ----
     constexpr uint32_t idesc_qk = instr_desc(kRows, kKeys, false);
     constexpr uint32_t idesc_pv = instr_desc(kRows, D, true);
-    const uint32_t elected = lane == 0 ? 1u : 0u;
+    const uint32_t elected = elect_one();
+    auto alike = [](uint32_t v) { return __shfl_sync(kFullMask, v, 0); };
     // the lower halves of the operands' descriptors; the upper ones are all alike
     const uint32_t q_desc = (uint32_t)smem_desc(q_smem, 16, 1024), k_desc = (uint32_t)smem_desc(k_smem, 16, 1024), v_desc = (uint32_t)smem_desc(v_smem, kBoxBytes, 1024);
     auto desc = [](uint32_t low) { return (uint64_t)low | (smem_desc(0, 0, 1024) & 0xffffffff00000000ull); };
@@ -320,7 +329,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       }
 #pragma unroll 1
       for (int e = 0; e < 2; ++e) {
-        const uint32_t s_at = tmem + 128u * e, o_at = tmem + 256u + (uint32_t)D * e;
+        const uint32_t s_at = alike(tmem + 128u * e), o_at = alike(tmem + 256u + (uint32_t)D * e);
         if (e < ne) {
           // O_e += P_e V once P_e is in tensor memory, on a segment's first tile once the last segment's O_e has been read; then at
           // once the next scores, which go where P_e lay
@@ -334,11 +343,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             o_used |= 1u << e;
           }
           tc_fence_after();
-          const uint32_t vd = v_desc + s * (kTileBytes >> 4);
+          const uint32_t vd = alike(v_desc + s * (kTileBytes >> 4));
+          if (elected) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk) mma_ts(o_at, s_at + kk * 8, desc(vd + kk * 128), idesc_pv, (!first || kk > 0) ? 1u : 0u, elected);
-          tc_commit(bar(O_FULL + e), elected);
-          if (e == ne - 1) tc_commit(bar(V_EMPTY + s), elected);
+            for (int kk = 0; kk < kKeys / 16; ++kk) mma_ts(o_at, s_at + kk * 8, desc(vd + kk * 128), idesc_pv, (!first || kk > 0) ? 1u : 0u, 1u);
+            tc_commit(bar(O_FULL + e), 1u);
+            if (e == ne - 1) tc_commit(bar(V_EMPTY + s), 1u);
+          }
+          __syncwarp();
         }
         if (on && e < nne) {
           if (e == 0) {
@@ -346,17 +358,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             if (nfirst && !mbar_wait_bounded(bar(Q_FULL), segments & 1)) { ok = false; break; }
             tc_fence_after();
           }
-          const uint32_t qd = q_desc + e * (kTileBytes >> 4), kd = k_desc + ns * (kTileBytes >> 4);
+          const uint32_t qd = alike(q_desc + e * (kTileBytes >> 4)), kd = alike(k_desc + ns * (kTileBytes >> 4));
+          if (elected) {
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t step = ((ks >> 2) * kBoxBytes + (ks & 3) * 32) / 16;
-            mma_ss(s_at, desc(qd + step), desc(kd + step), idesc_qk, ks > 0, elected);
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint32_t step = ((ks >> 2) * kBoxBytes + (ks & 3) * 32) / 16;
+              mma_ss(s_at, desc(qd + step), desc(kd + step), idesc_qk, ks > 0, 1u);
+            }
+            tc_commit(bar(S_FULL + e), 1u);
+            if (e == nne - 1) {
+              tc_commit(bar(K_EMPTY + ns), 1u);
+              if (nj + 1 == nj1) tc_commit(bar(Q_EMPTY), 1u);
+            }
           }
-          tc_commit(bar(S_FULL + e), elected);
-          if (e == nne - 1) {
-            tc_commit(bar(K_EMPTY + ns), elected);
-            if (nj + 1 == nj1) tc_commit(bar(Q_EMPTY), elected);
-          }
+          __syncwarp();
         }
       }
       // a round on

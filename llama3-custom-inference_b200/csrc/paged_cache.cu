@@ -4,7 +4,11 @@
 // Bound by the bytes of the rows, read once and written once.  One CTA per token: a thread owns one 16-byte vector of a head at a
 // time and sits at the same place of all its heads, so that it loads the rotary table and the norms' weights once; a head's sum of
 // squares is a shuffle over the lanes that hold it.  The row itself does not depend on where the token goes: its loads are asked for
-// before the chain starts -> positions -> page table, which is most of what a decode step's call takes.
+// before the chain starts -> positions -> page table, which is most of what a decode step's call takes.  With norms the arithmetic is near the
+// bytes' time as well (a warp has some 80 instructions a vector): the norms' weights go into the rotation, two floats an instruction.
+// Measured on a B200: 24 sequences, 20 with chunks of up to 500 tokens, 64 + 2 x 8 heads of 128 with norms, 294 MB: 55.7 us, 5.3 TB/s (62.7 before
+// those two); a prompt of 2001 tokens, 24 + 2 x 8 heads of 64 with norms, 20 MB mostly in L2: 8.3 us, two waves of CTAs; 64 single tokens: 6.2 us
+// a call back to back, which is the host's.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
