@@ -12,11 +12,12 @@
 //   * what lies behind a sequence's end in its last page, and values that some rows of a tile must not see, may be no numbers, and a
 //     weight of 0 does not stop them: two guard warps look through V tiles at the diagonal and the end, under the first product and the softmax
 //     of the same tile, take such values out, and the output group adds them to the rows that see them.
-// Measured on a B200: 2 x 512 tokens of 16500 keys, 32 query on 8 KV heads of 128, any page size 243 us, 1120 TFLOP/s, heads of 64 227, 600; a prompt of
-// 4096 tokens, heads of 128 155 us, 890, of 64 130, 530 (a head of 64 has half the products to the same exponentials).  A tile of keys takes
+// Measured on a B200: 2 x 512 tokens of 16500 keys, 32 query on 8 KV heads of 128, any page size 243 us, 1120 TFLOP/s, heads of 64 202, 675; a prompt of
+// 4096 tokens, heads of 128 155 us, 890, of 64 121, 570 (a head of 64 has half the products to the same exponentials).  A tile of keys takes
 // 3650 cycles (heads of 128), of which a warp's softmax is 2030 (its exponentials alone 1450 for the 1024 that they cannot do without) and
 // the wait for the products between 1240; the tensor cores need 2050 and the exponentials of both groups as much.  For heads of 64 the weights
-// in a place of their own, so that the next scores come under the exponentials: both groups then take theirs at once, 234 us instead of 227.
+// in a place of their own, so that the next scores come under the exponentials: both groups then take theirs at once, 234 us instead of 227 (of 202
+// with the first half of the weights multiplied ahead).
 // Scores read from tensor memory twice by loops of 32 keys instead of once: 3 to 10 % slower.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -69,6 +70,9 @@ template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                    const __grid_constant__ ChunkParams cp) {
+  // Whether the product of the first half of a tile's weights with their values starts under the exponentials of the second.  (Heads of 64 and of 128, 2 x 512
+  // tokens of 16500 keys: 227 us to 202, 243 either way and 1 % more at the power limit.)
+  constexpr bool kHalfWeights = D == 64;
   constexpr int kHalves = D / 64;
   constexpr int kBoxBytes = 128 * 128;             // 128 rows of 128 bytes
   constexpr int kTileBytes = kHalves * kBoxBytes;  // a Q, K or V tile
@@ -84,8 +88,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   uint64_t* bars = reinterpret_cast<uint64_t*>(stage_all + 2 * kRows * kSPitch);
   // as in prefill_tc_persist_kernel; V_OK: the guard warps have been through the tile, if it is one of theirs
   // (they arrive on V_EMPTY too, so that they never miss a phase of V_FULL)
-  enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_OK = 14, P_FULL = 16, L_FULL = 18, O_READ = 20,
-         SEG_FULL = 22, SEG_EMPTY = SEG_FULL + kSegments, N_BARS = SEG_EMPTY + kSegments };
+  enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_OK = 14, P_FULL = 16, L_FULL = 18, O_READ = 20, P_HALF = 22,
+         SEG_FULL = 24, SEG_EMPTY = SEG_FULL + kSegments, N_BARS = SEG_EMPTY + kSegments };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
   int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kSegments]: values taken out of tiles of a segment
   int* sums = odd + kSegments;                                            // [16 warps]
@@ -333,8 +337,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (e < ne) {
           // O_e += P_e V once P_e is in tensor memory, on a segment's first tile once the last segment's O_e has been read; then at
           // once the next scores, which go where P_e lay
-          if (!mbar_wait_bounded(bar(P_FULL + e), (p_phase >> e) & 1)) { ok = false; break; }
-          p_phase ^= 1u << e;
+          if (!mbar_wait_bounded(bar((kHalfWeights ? P_HALF : P_FULL) + e), (p_phase >> e) & 1)) { ok = false; break; }
           if (first) {
             if ((o_used >> e) & 1) {
               if (!mbar_wait_bounded(bar(O_READ + e), (o_phase >> e) & 1)) { ok = false; break; }
@@ -344,9 +347,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
           tc_fence_after();
           const uint32_t vd = alike(v_desc + s * (kTileBytes >> 4));
+          constexpr int kFirst = kKeys / 16 / (kHalfWeights ? 2 : 1);
           if (elected) {
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk) mma_ts(o_at, s_at + kk * 8, desc(vd + kk * 128), idesc_pv, (!first || kk > 0) ? 1u : 0u, 1u);
+            for (int kk = 0; kk < kFirst; ++kk) mma_ts(o_at, s_at + kk * 8, desc(vd + kk * 128), idesc_pv, (!first || kk > 0) ? 1u : 0u, 1u);
+          }
+          __syncwarp();
+          if constexpr (kHalfWeights) {
+            if (!mbar_wait_bounded(bar(P_FULL + e), (p_phase >> e) & 1)) { ok = false; break; }
+            tc_fence_after();
+          }
+          p_phase ^= 1u << e;
+          if (elected) {
+#pragma unroll
+            for (int kk = kFirst; kk < kKeys / 16; ++kk) mma_ts(o_at, s_at + kk * 8, desc(vd + kk * 128), idesc_pv, 1u, 1u);
             tc_commit(bar(O_FULL + e), 1u);
             if (e == ne - 1) tc_commit(bar(V_EMPTY + s), 1u);
           }
@@ -522,6 +536,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
               pk[i] = pack_bf16x2(pe[2 * i], pe[2 * i + 1]);
             }
             tmem_st16(ts + c * 16, pk);                // P: 64 packed columns over the first 64 of S
+            if (kHalfWeights && c == 1) {
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(P_HALF + e));
+            }
           }
           {
             float a0, a1, b0, b1;
@@ -670,7 +690,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 // ---- host ----
 size_t chunk_smem(int D, int B) {
   const size_t tile = (size_t)(D / 64) * 128 * 128;
-  return 1024 + 6 * tile + 2 * kRows * 80 + (23 + 2 * kSegments) * 8 + (kSegments + 16) * 4 + 4 * kRows * 4 + kSegments * sizeof(Segment) + (size_t)(B + 1) * 4;
+  return 1024 + 6 * tile + 2 * kRows * 80 + (25 + 2 * kSegments) * 8 + (kSegments + 16) * 4 + 4 * kRows * 4 + kSegments * sizeof(Segment) + (size_t)(B + 1) * 4;
 }
 
 int chunk_parts(const PagedParams& p) {
