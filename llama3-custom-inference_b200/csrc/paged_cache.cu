@@ -7,10 +7,12 @@
 // before the chain starts -> positions -> page table, which is most of what a decode step's call takes.  With norms the arithmetic is near the
 // bytes' time as well (a warp has some 80 instructions a vector): the norms' weights go into the rotation, two floats an instruction.
 // Measured on a B200: 24 sequences, 20 with chunks of up to 500 tokens, 64 + 2 x 8 heads of 128 with norms, 294 MB: 55.7 us, 5.3 TB/s (62.7 before
-// those two); a prompt of 2001 tokens, 24 + 2 x 8 heads of 64 with norms, 20 MB mostly in L2: 8.3 us, two waves of CTAs; 64 single tokens: 6.2 us
-// a call back to back, which is the host's.
+// those two); a prompt of 2001 tokens, 24 + 2 x 8 heads of 64 with norms, 20 MB mostly in L2: 5.2 us, one wave of CTAs; 64 single tokens of 32 + 2 x 8
+// heads of 128: 2.4 us in a graph, 6.2 in calls from the host, whose time that is.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "bf16x8.cuh"
 #include "host_common.h"
@@ -22,7 +24,6 @@
 namespace l3ci {
 namespace {
 
-constexpr int kBlock = 128;
 constexpr int kBatch = 4;   // 16-byte loads of queries a thread has in flight
 
 typedef unsigned long long f2;   // two floats
@@ -70,8 +71,8 @@ __device__ __forceinline__ uint4 norm_rotate8(const uint4& v, const Turn& t, flo
 }
 
 // LANES: lanes that hold a head, a power of two of at least D / 8 (those beyond it have nothing).
-template <int LANES, bool NORM>
-__global__ void __launch_bounds__(kBlock, NORM ? 7 : 9)
+template <int LANES, bool NORM, int kBlock>
+__global__ void __launch_bounds__(kBlock, (NORM ? 7 : 9) * 128 / kBlock)
 rot_embed_paged_kv_cache_kernel(const l3ci_paged_rope_args p) {
   __shared__ int found;
   if (threadIdx.x == 0) found = -1;
@@ -179,11 +180,26 @@ extern "C" int l3ci_rot_embed_paged_kv_cache(const l3ci_paged_rope_args* a) {
     return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: tensor too large");
   if (rows > 1 && a->q_st < (long long)a->Hq * a->D) return fail(L3CI_ERR_INVALID, "rot_embed_paged_kv_cache: rows of the queries overlap");
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
-  auto go = [&](auto kernel) -> int {
-    L3CI_LAUNCH("rot_embed_paged_kv_cache_kernel", kernel, dim3((unsigned)rows), dim3(kBlock), 0, stream, *a);
-    return L3CI_OK;
+  auto go = [&](auto lanes, auto norm) -> int {
+    constexpr int kLanes = decltype(lanes)::value;
+    constexpr bool kNorm = decltype(norm)::value;
+    auto in = [&](auto threads) -> int {
+      constexpr int kBlock = decltype(threads)::value;
+      L3CI_LAUNCH("rot_embed_paged_kv_cache_kernel", (rot_embed_paged_kv_cache_kernel<kLanes, kNorm, kBlock>), dim3((unsigned)rows), dim3(kBlock), 0, stream, *a);
+      return L3CI_OK;
+    };
+    // The smallest CTA that asks for its whole row before it waits.  (Threads without a vector keep others off the SM: 2001 tokens of 24 + 2 x 8 heads of 64
+    // with norms take 8.2 us by CTAs of 128, 5.2 by 64, 6.4 by 32; 6000 of 16 + 2 heads of 64 19.6, 11.6, 8.2; of 32 + 2 x 8 heads of 128 30.3, 29.2, 30.8,
+    // a single token of these 3.0, 4.2, 6.5.)
+    auto holds = [&](int threads) { return a->Hq * kLanes <= threads * kBatch && a->Hkv * kLanes <= threads; };
+    if (holds(32)) return in(std::integral_constant<int, 32>{});
+    if (holds(64)) return in(std::integral_constant<int, 64>{});
+    // (where every CTA has an SM of its own: 64 tokens of 64 + 2 x 8 heads of 128 2.3 us instead of 3.0; 500 of them with norms 6.6 and 5.5)
+    if (!holds(128) && holds(256) && rows <= sm_count()) return in(std::integral_constant<int, 256>{});
+    return in(std::integral_constant<int, 128>{});
   };
-  if (a->D <= 64) return a->q_norm ? go(rot_embed_paged_kv_cache_kernel<8, true>) : go(rot_embed_paged_kv_cache_kernel<8, false>);
-  if (a->D <= 128) return a->q_norm ? go(rot_embed_paged_kv_cache_kernel<16, true>) : go(rot_embed_paged_kv_cache_kernel<16, false>);
-  return a->q_norm ? go(rot_embed_paged_kv_cache_kernel<32, true>) : go(rot_embed_paged_kv_cache_kernel<32, false>);
+  auto with = [&](auto lanes) { return a->q_norm ? go(lanes, std::true_type{}) : go(lanes, std::false_type{}); };
+  if (a->D <= 64) return with(std::integral_constant<int, 8>{});
+  if (a->D <= 128) return with(std::integral_constant<int, 16>{});
+  return with(std::integral_constant<int, 32>{});
 }
