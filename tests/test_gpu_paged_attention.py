@@ -84,6 +84,17 @@ def test_queries_that_are_broadcast(ext, device, new):
     check(got, case)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_sequences_that_share_pages_and_results_in_the_place_of_queries(ext, device, D):
+    case = attention_case([1, 90, 3, 1], [700, 690, 803, 640], 8, 2, D, 16, device, seed=D)
+    case.table[1:, :30] = case.table[0, :30]          # 480 tokens in common
+    apart = run(ext, case)
+    check(apart, case)
+    case.rows = case.q.clone()
+    assert run(ext, case, out=case.q) is not None
+    assert torch.equal(case.q, apart)
+
+
 def test_lengths_that_leave_tokens_without_keys(ext, device):
     # fewer tokens cached than are new: the first ones see nothing; a length of zero; one beyond the table's row is clamped
     case = attention_case([5, 40, 3, 1, 300], [64, 64, 64, 64, 320], 8, 2, 128, 16, device, seed=9)
