@@ -6,7 +6,7 @@
 // squares is a shuffle over the lanes that hold it.  The row itself does not depend on where the token goes: its loads are asked for
 // before the chain starts -> positions -> page table, which is most of what a decode step's call takes.  With norms the arithmetic is near the
 // bytes' time as well (a warp has some 80 instructions a vector): the norms' weights go into the rotation, two floats an instruction.
-// Measured on a B200: 24 sequences, 20 with chunks of up to 500 tokens, 64 + 2 x 8 heads of 128 with norms, 294 MB: 55.7 us, 5.3 TB/s (62.7 before
+// Measured on a B200: 24 sequences, 20 with chunks of up to 500 tokens, 64 + 2 x 8 heads of 128 with norms, 294 MB: 53.8 us, 5.5 TB/s (62.7 before
 // those two); a prompt of 2001 tokens, 24 + 2 x 8 heads of 64 with norms, 20 MB mostly in L2: 5.2 us, one wave of CTAs; 64 single tokens of 32 + 2 x 8
 // heads of 128: 2.4 us in a graph, 6.2 in calls from the host, whose time that is.
 #include <cuda_bf16.h>
