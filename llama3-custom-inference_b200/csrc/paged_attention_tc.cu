@@ -91,7 +91,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, O_FULL = 11, Q_EMPTY = 13, V_OK = 14, P_FULL = 16, L_FULL = 18, O_READ = 20, P_HALF = 22,
          SEG_FULL = 24, SEG_EMPTY = SEG_FULL + kSegments, N_BARS = SEG_EMPTY + kSegments };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
-  int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kSegments]: values taken out of tiles of a segment
+  int* odd = reinterpret_cast<int*>(bars + N_BARS + 1);            // [kSegments]: one more than the number of the last segment of which values were taken out
   int* sums = odd + kSegments;                                            // [16 warps]
   float* stat = reinterpret_cast<float*>(sums + 16);               // [2 tiles][128 rows][l, m_ref]
   Segment* segs = reinterpret_cast<Segment*>(stat + 4 * kRows);    // [kSegments]
@@ -439,7 +439,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             if (write) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
           }
         }
-        if (any) odd[segments % kSegments] = 1;
+        if (any) odd[segments % kSegments] = segments + 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -565,7 +565,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOut));
-    // ---- output: a thread a row of one tile after the other ----
+    // ---- output: a thread a row of one tile after the other.  No barrier among the four warps: each finds out for itself when a wait has run out, and the
+    // others would stand at it for good ----
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(q4 * 32) << 16;
     int g[2] = {0, 0}, mine[2] = {0, 0};
@@ -584,7 +585,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (!mbar_wait_bounded(bar(O_FULL + e), (g[e] - 1) & 1)) { ok = false; break; }   // the segment's last product
         tc_fence_after();
         const int t0 = s.t0 + e * cp.tile_tokens, tokens = min(cp.tile_tokens, s.n - t0);   // tokens of the tile
-        const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kSegments) != 0;
+        const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kSegments) == segments + 1;
         const float inv = lm.x == 0.f ? 0.f : 1.f / lm.x;
         float* rec = chunk_part_of<D>(p, part, j0 == 0);
         const uint32_t to = t_o[e] + lane_addr;
@@ -613,10 +614,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
         }
         auto read = [&]() {                                   // O_e and the row's sums are in registers: they may take the next segment's
-          if (e == ne - 1) {
-            asm volatile("bar.sync 2, 128;" ::: "memory");    // (all have read the mark)
-            if (r == 0) odd[segments % kSegments] = 0;
-          }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(O_READ + e));
