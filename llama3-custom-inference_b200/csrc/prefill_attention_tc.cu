@@ -953,10 +953,15 @@ prefill_tc_persist_kernel(const __grid_constant__ CUtensorMap qmap, const __grid
       if (!it.valid) break;
       const int m0 = it.m0;
       for (int e = 0; e < 2 && ok; ++e) {
-        if (!mbar_wait_bounded(bar(L_FULL + e), round & 1)) { ok = false; break; }
+        ok = mbar_wait_bounded(bar(L_FULL + e), round & 1) && mbar_wait_bounded(bar(O_FULL + e), (g0 + it.n_tiles - 1) & 1);   // the head's last product
+        {   // (the four warps go on together or not at all: one alone would leave the others at the barriers below)
+          uint32_t all;
+          asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+          ok = all != 0;
+        }
+        if (!ok) break;
         const float l_all = lrow[e * kTcRows + r];
         const float inv = l_all > 0.f ? 1.f / l_all : 0.f;
-        if (!mbar_wait_bounded(bar(O_FULL + e), (g0 + it.n_tiles - 1) & 1)) { ok = false; break; }   // the head's last product
         tc_fence_after();
         // 32 columns at a time through the staging rows (a thread holds one row; stored straight to global memory
         // every store instruction of a warp would touch 32 rows): out of tensor memory, scaled, packed, into shared

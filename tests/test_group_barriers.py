@@ -44,6 +44,6 @@ def test_the_check_itself():
     assert left_alone(loop.replace("  for (;;) {\n", "  for (;;) {\n  }\n  {\n")) == []
 
 
-@pytest.mark.parametrize("name", ["paged_attention_tc.cu"])
+@pytest.mark.parametrize("name", sorted(p.name for p in CSRC.glob("*.cu")))
 def test_no_warp_leaves_the_others_at_a_barrier(name):
     assert left_alone((CSRC / name).read_text()) == []
