@@ -47,7 +47,8 @@ L3CI_API const char* l3ci_last_error(void);
 L3CI_API const char* l3ci_version(void);
 
 /* Bound of the device-side waits on OTHER CTAs or OTHER GPUs (the arrival counters of l3ci_flash_decode's
- * persistent kernel, default 2 s; the peers' flags of l3ci_lse_exchange_merge, default 1 s), in nanoseconds,
+ * persistent kernel, default 2 s; the peers' flags of l3ci_lse_exchange_merge, default 1 s) and of the waits in l3ci_paged_attention's
+ * kernel of chunks (default 2 s, at most 4 s; some last as long as a block's run of one sequence's keys, 2 us for 128), in nanoseconds,
  * for the launches made after this call by any thread of the process; 0 restores the defaults.  Returns the
  * previous setting.  A wait that runs out makes the kernel give up in order: it records
  * L3CI_ERR_DEVICE_WAIT (scratch header / status word), skips the rows it could not finish and returns,

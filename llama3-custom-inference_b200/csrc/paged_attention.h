@@ -58,6 +58,7 @@ struct ChunkParams {
   int tile_tokens;   // tokens of a tile of query rows: 128 / R
   int box;           // tokens of a copy
   int follows;       // launched behind paged_rows_kernel of the same call, which has waited for the kernels before
+  uint32_t wait_ns;  // bound of every wait
 };
 // Floats of a part: o[D / 4][256 rows][4], m[256], l[256].
 constexpr long long chunk_part_floats(int D) { return 2 * kChunkRows * (D + 2); }

@@ -98,6 +98,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   int* pref = reinterpret_cast<int*>(segs + kSegments);            // [B + 1]
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
+  auto wait = [&](uint32_t at, uint32_t parity) { return mbar_wait_bounded_lo(at, parity, cp.wait_ns); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -158,7 +159,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   auto take = [&](int k) {
     __syncwarp();
     if (k > 0 && lane == 0) mbar_arrive(bar(SEG_EMPTY + (k - 1) % kSegments));
-    return mbar_wait_bounded(bar(SEG_FULL + k % kSegments), (k / kSegments) & 1);
+    return wait(bar(SEG_FULL + k % kSegments), (k / kSegments) & 1);
   };
   auto cut_tile = [&](int j, int limit) { return j * kKeys + kKeys - 1 > limit; };    // some row does not see all keys
   bool ok = true;
@@ -242,7 +243,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const int copies = kKeys / cp.box;                      // per half of a tile
     for (;; ++segments) {
       const int slot = segments % kSegments;
-      if (segments >= kSegments && !mbar_wait_bounded(bar(SEG_EMPTY + slot), (segments / kSegments - 1) & 1)) { ok = false; break; }
+      if (segments >= kSegments && !wait(bar(SEG_EMPTY + slot), (segments / kSegments - 1) & 1)) { ok = false; break; }
       const int j0 = tiles_from(u, col), j1 = on ? min(u.tiles, tiles_from(u, end)) : 0;
       const int row = a.starts && on ? __ldg(a.starts + u.b) : 0;
       const bool two = (u.m * 2 + 1) * cp.tile_tokens < u.n;
@@ -268,10 +269,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) tma_load_4d(to + s * kTileBytes + h * kBoxBytes + lane * cp.box * 128, &map, full, h * 64, off, u.h, page, policy);
         };
-        if (fill >= kStages && !mbar_wait_bounded(bar(K_EMPTY + s), par)) { ok = false; break; }
+        if (fill >= kStages && !wait(bar(K_EMPTY + s), par)) { ok = false; break; }
         load(kmap, k_smem, bar(K_FULL + s));
         if (j == j0) {     // (behind the first keys, whose place is free before the last unit's scores are done)
-          if (segments > 0 && !mbar_wait_bounded(bar(Q_EMPTY), (segments - 1) & 1)) { ok = false; break; }
+          if (segments > 0 && !wait(bar(Q_EMPTY), (segments - 1) & 1)) { ok = false; break; }
           if (lane == 0) {
             const int tiles = two ? 2 : 1;
             mbar_expect_tx(bar(Q_FULL), tiles * kHalves * cp.tile_tokens * p.R * 128);
@@ -281,7 +282,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
                 tma_load_4d(q_smem + e * kTileBytes + h * kBoxBytes, &qmap, bar(Q_FULL), h * 64, u.h * p.R, row + u.m * block + e * cp.tile_tokens, a.starts ? 0 : u.b, policy);
           }
         }
-        if (fill >= kStages && !mbar_wait_bounded(bar(V_EMPTY + s), par)) { ok = false; break; }
+        if (fill >= kStages && !wait(bar(V_EMPTY + s), par)) { ok = false; break; }
         load(vmap, v_smem, bar(V_FULL + s));
         page = ahead;
       }
@@ -325,9 +326,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     for (fill = -1; (on || ne > 0) && ok; ++fill) {
       const int s = fill & (kStages - 1), ns = (fill + 1) & (kStages - 1);
       if (ne > 0) {
-        if (!mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
+        if (!wait(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
         if (cut_tile(j, limit)) {
-          if (!mbar_wait_bounded(bar(V_OK + s), (guarded >> s) & 1)) { ok = false; break; }
+          if (!wait(bar(V_OK + s), (guarded >> s) & 1)) { ok = false; break; }
           guarded ^= 1u << s;
         }
       }
@@ -337,10 +338,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (e < ne) {
           // O_e += P_e V once P_e is in tensor memory, on a segment's first tile once the last segment's O_e has been read; then at
           // once the next scores, which go where P_e lay
-          if (!mbar_wait_bounded(bar((kHalfWeights ? P_HALF : P_FULL) + e), (p_phase >> e) & 1)) { ok = false; break; }
+          if (!wait(bar((kHalfWeights ? P_HALF : P_FULL) + e), (p_phase >> e) & 1)) { ok = false; break; }
           if (first) {
             if ((o_used >> e) & 1) {
-              if (!mbar_wait_bounded(bar(O_READ + e), (o_phase >> e) & 1)) { ok = false; break; }
+              if (!wait(bar(O_READ + e), (o_phase >> e) & 1)) { ok = false; break; }
               o_phase ^= 1u << e;
             }
             o_used |= 1u << e;
@@ -354,7 +355,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
           __syncwarp();
           if constexpr (kHalfWeights) {
-            if (!mbar_wait_bounded(bar(P_FULL + e), (p_phase >> e) & 1)) { ok = false; break; }
+            if (!wait(bar(P_FULL + e), (p_phase >> e) & 1)) { ok = false; break; }
             tc_fence_after();
           }
           p_phase ^= 1u << e;
@@ -368,8 +369,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         if (on && e < nne) {
           if (e == 0) {
-            if (!mbar_wait_bounded(bar(K_FULL + ns), ((fill + 1) / kStages) & 1)) { ok = false; break; }
-            if (nfirst && !mbar_wait_bounded(bar(Q_FULL), segments & 1)) { ok = false; break; }
+            if (!wait(bar(K_FULL + ns), ((fill + 1) / kStages) & 1)) { ok = false; break; }
+            if (nfirst && !wait(bar(Q_FULL), segments & 1)) { ok = false; break; }
             tc_fence_after();
           }
           const uint32_t qd = alike(q_desc + e * (kTileBytes >> 4)), kd = alike(k_desc + ns * (kTileBytes >> 4));
@@ -415,7 +416,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       if (j1 == 0) break;
       for (int j = g.j0; j < j1 && ok; ++j, ++fill) {
         const int s = fill % kStages;
-        if (!mbar_wait_bounded(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
+        if (!wait(bar(V_FULL + s), (fill / kStages) & 1)) { ok = false; break; }
         if (!cut_tile(j, limit)) {
           if (lane == 0) mbar_arrive(bar(V_EMPTY + s));
           continue;
@@ -467,7 +468,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const int limit = token < cp.tile_tokens ? min(limit0 + token, s.len - 1) : -1;   // last key this row may see
         float m_ref = -INFINITY, l_run = 0.f;
         for (int j = j0; j < j1 && ok; ++j, ++g) {
-          if (!mbar_wait_bounded(bar(S_FULL + e), g & 1)) { ok = false; break; }
+          if (!wait(bar(S_FULL + e), g & 1)) { ok = false; break; }
           tc_fence_after();
           uint32_t x[4][32];
 #pragma unroll
@@ -493,7 +494,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             const float m_new = fmaxf(m_ref, mx);
             const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
             if (j > j0) {
-              if (!mbar_wait_bounded(bar(O_FULL + e), (g - 1) & 1)) { ok = false; break; }
+              if (!wait(bar(O_FULL + e), (g - 1) & 1)) { ok = false; break; }
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
@@ -556,7 +557,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         if (!ok) break;
         // the row's sums go to the output group, which has read the last segment's before it arrived on O_READ
-        if (mine > 0 && !mbar_wait_bounded(bar(O_READ + e), (mine - 1) & 1)) { ok = false; break; }
+        if (mine > 0 && !wait(bar(O_READ + e), (mine - 1) & 1)) { ok = false; break; }
         *reinterpret_cast<float2*>(stat + (e * kRows + r) * 2) = make_float2(l_run, m_ref);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(L_FULL + e));
@@ -579,10 +580,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const bool whole = s.whole != 0;
       const long long row0 = a.starts ? s.row * a.o_st : s.b * a.o_sb;
       for (int e = 0; e < ne && ok; ++e) {
-        if (!mbar_wait_bounded(bar(L_FULL + e), mine[e] & 1)) { ok = false; break; }
+        if (!wait(bar(L_FULL + e), mine[e] & 1)) { ok = false; break; }
         const float2 lm = *reinterpret_cast<const float2*>(stat + (e * kRows + r) * 2);
         g[e] += j1 - j0;
-        if (!mbar_wait_bounded(bar(O_FULL + e), (g[e] - 1) & 1)) { ok = false; break; }   // the segment's last product
+        if (!wait(bar(O_FULL + e), (g[e] - 1) & 1)) { ok = false; break; }   // the segment's last product
         tc_fence_after();
         const int t0 = s.t0 + e * cp.tile_tokens, tokens = min(cp.tile_tokens, s.n - t0);   // tokens of the tile
         const bool taken = *reinterpret_cast<volatile int*>(odd + segments % kSegments) == segments + 1;
@@ -672,12 +673,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   if (cp.follows) pdl_wait();              // (the merge behind counts on both kernels)
   __syncwarp();
   tc_fence_before();
-  // a wait ran out: the copies still under way land before the shared memory is given back (or their own waits run out too)
-  if (__syncthreads_or(!ok) && threadIdx.x == 0) {
-    if (segments > 0 || fill > 0) (void)mbar_wait_bounded_one(bar(Q_FULL), segments & 1);
-    for (int f = max(fill - kStages, 0); f <= fill; ++f) {
-      (void)mbar_wait_bounded_one(bar(K_FULL + f % kStages), (f / kStages) & 1);
-      (void)mbar_wait_bounded_one(bar(V_FULL + f % kStages), (f / kStages) & 1);
+  // a wait ran out: the copies and the products still under way end before the shared and the tensor memory are given back (or their own waits run out too)
+  if (__syncthreads_or(!ok) && (threadIdx.x == 0 || warp == 1)) {
+    if (threadIdx.x == 0) {
+      if (segments > 0 || fill > 0) (void)mbar_wait_bounded_one(bar(Q_FULL), segments & 1, cp.wait_ns);
+      for (int f = max(fill - kStages, 0); f <= fill; ++f) {
+        (void)mbar_wait_bounded_one(bar(K_FULL + f % kStages), (f / kStages) & 1, cp.wait_ns);
+        (void)mbar_wait_bounded_one(bar(V_FULL + f % kStages), (f / kStages) & 1, cp.wait_ns);
+      }
+    } else if (elect_one()) {              // (the lane that issued the products, on a barrier that nobody has to do with any more)
+      const uint32_t at = bar(SEG_EMPTY);
+      asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(at) : "memory");
+      mbar_init(at, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_commit(at, 1u);
+      (void)mbar_wait_bounded_one(at, 0, cp.wait_ns);
     }
   }
   __syncthreads();
@@ -763,6 +774,8 @@ int paged_chunks_launch(const PagedParams& params, void* scratch, bool follows, 
   const int low = params.a.page_size & -params.a.page_size;    // tokens that lie together in every page: a power of two
   cp.box = low < kKeys ? low : kKeys;
   cp.follows = follows;
+  const unsigned long long limit = device_wait_limit_ns(kWaitLimitNs);
+  cp.wait_ns = limit < kWaitLimitLoNs ? (uint32_t)limit : kWaitLimitLoNs;
   return params.a.D == 64 ? chunk_launch<64>(cp, stream) : chunk_launch<128>(cp, stream);
 }
 
