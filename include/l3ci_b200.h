@@ -443,7 +443,7 @@ typedef struct l3ci_paged_attention_args {
   const int32_t *page_table, *seq_lens, *starts;
   void* scratch;
   size_t scratch_bytes;
-  int32_t* status;             /* optional device word: L3CI_ERR_DEVICE_WAIT when a bounded wait runs out                */
+  int32_t* status;             /* device word: L3CI_ERR_DEVICE_WAIT when a bounded wait runs out, out is then not complete; null: a word of the library's */
   int64_t rows;
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, pages, cache_sp, cache_st, table_st;
   int32_t B, T, Hq, Hkv, D, page_size, max_pages;
@@ -453,6 +453,10 @@ typedef struct l3ci_paged_attention_args {
 L3CI_API int l3ci_paged_attention(const l3ci_paged_attention_args* args);
 /* Bytes of scratch the call wants on the current device (0: none, or sizes that the call would refuse). */
 L3CI_API size_t l3ci_paged_attention_scratch_bytes(const l3ci_paged_attention_args* args);
+
+/* Waits for `stream`; L3CI_ERR_DEVICE_WAIT, once, if a launch of l3ci_paged_attention without a status word of its own gave up on this device (should never
+ * happen). */
+L3CI_API int l3ci_paged_attention_poll(l3ci_stream_t stream);
 
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[r] = x[r] w^T + scales[i] (x[r] a[i]^T) b[i]^T,   i = index[r];   i outside [0, adapters): the shared product alone.

@@ -36,6 +36,9 @@
 namespace l3ci {
 namespace {
 
+// Where a wait that ran out is recorded by calls without a status word of their own, until l3ci_paged_attention_poll reads it.
+__device__ int g_wait_status = 0;
+
 constexpr int kRows = kChunkRows;   // query rows of a tile (M of the products)
 constexpr int kKeys = 128;     // keys of a tile
 constexpr int kStages = 2;
@@ -669,7 +672,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       }
     }
   }
-  if (!ok && lane == 0 && a.status) atomicExch(a.status, (int)L3CI_ERR_DEVICE_WAIT);
+  if (!ok && lane == 0) atomicExch(a.status ? a.status : &g_wait_status, (int)L3CI_ERR_DEVICE_WAIT);
   if (cp.follows) pdl_wait();              // (the merge behind counts on both kernels)
   __syncwarp();
   tc_fence_before();
@@ -780,3 +783,18 @@ int paged_chunks_launch(const PagedParams& params, void* scratch, bool follows, 
 }
 
 }  // namespace l3ci
+
+extern "C" int l3ci_paged_attention_poll(l3ci_stream_t stream_) {
+  using namespace l3ci;
+  clear_error();
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  void* word = nullptr;
+  int status = 0;
+  L3CI_CUDA_TRY(cudaGetSymbolAddress(&word, g_wait_status));
+  L3CI_CUDA_TRY(cudaMemcpyAsync(&status, word, sizeof(int), cudaMemcpyDeviceToHost, stream));
+  L3CI_CUDA_TRY(cudaStreamSynchronize(stream));
+  if (status == 0) return L3CI_OK;
+  L3CI_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), stream));
+  L3CI_CUDA_TRY(cudaStreamSynchronize(stream));
+  return fail(status, "paged_attention: a bounded wait ran out in an earlier launch");
+}

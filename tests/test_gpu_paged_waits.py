@@ -50,3 +50,19 @@ def test_waits_that_run_out_end_the_call_and_are_reported(ext, capi, device, D, 
     assert int(status) == capi.ERR_DEVICE_WAIT
     assert torch.equal(go(), want)
     del held
+
+
+def test_the_extension_reports_them_once(ext, capi, device):
+    D, keys = 64, torch.cuda.get_device_properties(device).multi_processor_count * 12000 * 128 // PAGE * PAGE
+    k, v = (torch.randn(1, PAGE, 1, D, device=device).to(BF16) for _ in range(2))
+    q = torch.randn(1, 16, 16, D, device=device).to(BF16)
+    table = torch.zeros(1, keys // PAGE, dtype=torch.int32, device=device)
+    lens = torch.tensor([PAGE], dtype=torch.int32, device=device)
+    want = ext.paged_attention(q, k, v, table, lens)
+    assert ext.paged_attention_status(q) == capi.OK
+    with capi.device_wait_limit(LIMIT_NS):
+        ext.paged_attention(q, k, v, table, lens * (keys // PAGE))
+        torch.cuda.synchronize()
+    assert ext.paged_attention_status(q) == capi.ERR_DEVICE_WAIT
+    assert ext.paged_attention_status(q) == capi.OK
+    assert torch.equal(ext.paged_attention(q, k, v, table, lens), want) and ext.paged_attention_status(q) == capi.OK
