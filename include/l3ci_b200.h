@@ -479,6 +479,9 @@ typedef struct l3ci_adapter_linear_args {
 } l3ci_adapter_linear_args;
 L3CI_API int l3ci_adapter_linear(const l3ci_adapter_linear_args* args);
 L3CI_API size_t l3ci_adapter_linear_scratch_bytes(const l3ci_adapter_linear_args* args);
+/* Which product l3ci_adapter_linear takes on the current device for these sizes: 0 that of few rows, 1 that of many; -1 where the call would be refused or
+ * has nothing to do.  For tests and measurements; a fit that may change between versions. */
+L3CI_API int l3ci_adapter_linear_kernel_choice(const l3ci_adapter_linear_args* args);
 
 #ifdef __cplusplus
 }

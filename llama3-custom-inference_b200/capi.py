@@ -25,7 +25,7 @@ EXPORTS = (
     "l3ci_lse_merge", "l3ci_lse_exchange_bytes", "l3ci_lse_exchange_merge", "l3ci_prefill_attention",
     "l3ci_flash_decode_exchange_bytes", "l3ci_flash_decode_exchange",
     "l3ci_rot_embed_paged_kv_cache", "l3ci_paged_attention", "l3ci_paged_attention_scratch_bytes", "l3ci_paged_attention_poll",
-    "l3ci_adapter_linear", "l3ci_adapter_linear_scratch_bytes",
+    "l3ci_adapter_linear", "l3ci_adapter_linear_scratch_bytes", "l3ci_adapter_linear_kernel_choice",
 )
 
 
@@ -180,6 +180,8 @@ def load() -> C.CDLL:
     lib.l3ci_paged_attention_poll.argtypes = [vp]
     lib.l3ci_adapter_linear_scratch_bytes.restype = C.c_size_t
     lib.l3ci_adapter_linear_scratch_bytes.argtypes = [C.POINTER(AdapterLinearArgs)]
+    lib.l3ci_adapter_linear_kernel_choice.restype = C.c_int
+    lib.l3ci_adapter_linear_kernel_choice.argtypes = [C.POINTER(AdapterLinearArgs)]
     _lib = lib
     return lib
 

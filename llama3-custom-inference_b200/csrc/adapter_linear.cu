@@ -243,6 +243,12 @@ extern "C" size_t l3ci_adapter_linear_scratch_bytes(const l3ci_adapter_linear_ar
   return st ? 0 : l3ci::scratch_of(a);
 }
 
+extern "C" int l3ci_adapter_linear_kernel_choice(const l3ci_adapter_linear_args* a) {
+  const int st = l3ci::check(a);
+  l3ci::clear_error();
+  return st ? -1 : l3ci::few_rows(a) ? 0 : 1;
+}
+
 extern "C" int l3ci_adapter_linear(const l3ci_adapter_linear_args* a) {
   using namespace l3ci;
   clear_error();
