@@ -1,4 +1,5 @@
-"""Low-rank adapters beside the product of many rows: the tests of test_gpu_adapters.py at sizes that this product takes (each test asks which one does).
+"""Low-rank adapters beside the product of many rows: the tests of test_gpu_adapters.py at sizes that this product takes (each test asks which one does),
+and what a rounding of the low-rank factor would cost.
 
 Tolerance: as there."""
 import ctypes as C
@@ -9,7 +10,7 @@ import torch
 from test_gpu_adapters import BF16, check, make, spread
 
 pytestmark = pytest.mark.gpu
-MANY = 1
+FEW, MANY = 0, 1
 # (rows, K, N): the first factor row by row (up to 512) and by tiles of rows beyond; the last tile of 256 rows and of 256 columns half empty
 SIZES = [(500, 264, 2056), (2049, 264, 520)]
 RANKS = [8, 16, 24, 32, 40, 64, 72, 104, 128]
@@ -103,3 +104,31 @@ def test_same_bits_on_another_stream_and_in_graphs_at_once(ext, capi, device, ro
             graphs[1].replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("rank", [16, 40])
+@pytest.mark.parametrize("rows,K,N,product", [(40, 264, 520, FEW), (500, 264, 2056, MANY), (2049, 264, 520, MANY)])
+def test_the_low_rank_factor_keeps_more_than_eight_bits(ext, capi, device, rank, rows, K, N, product):
+    # w = 0, and z = u + 2^-8 v of bf16 u and v in [1, 2): 16 bits.  Pairs of ranks share u and meet b = 1 and -1, so that the results are the sums of
+    # 2^-8 (v - v'), of which a z of eight bits keeps nothing.  All terms are multiples of 2^-15, all sums below 2^7: 32 bits hold them, and the
+    # results are off by their rounding; 2^-17 of the sum of |z b|, half of what two bf16 may lose of z, is allowed beside it.
+    g = torch.Generator().manual_seed(rank + rows)
+    c = make(device, rows, K, N, rank, 3, spread(rows, 3), seed=1)
+    assert takes(capi, c) == product
+    eighths = lambda *s: 1 + torch.randint(0, 128, s, generator=g) / 128  # noqa: E731
+    c["scales"] = None
+    c["w"].zero_(), c["x"].zero_(), c["a"].zero_()
+    c["x"][:, 0], c["x"][:, K - 1] = 1.0, 2.0 ** -8
+    c["a"][:, :, 0] = eighths(3, rank // 2).repeat_interleave(2, dim=1).to(BF16).to(device)
+    c["a"][:, :, K - 1] = eighths(3, rank).to(BF16).to(device)
+    sign = torch.tensor([1.0, -1.0], device=device).repeat(rank // 2).to(BF16)
+    c["b"].copy_(sign.expand_as(c["b"]))
+    got = ext.adapter_linear(**c).double()
+    z = (c["a"][:, :, 0].double() + 2.0 ** -8 * c["a"][:, :, K - 1].double())
+    want = torch.zeros(rows, dtype=torch.float64, device=device)
+    mine = c["index"] >= 0
+    want[mine] = (z * sign.double()).sum(1)[c["index"][mine].long()]
+    bound = want.abs() * 2 ** -8 + 2 ** -17 * z.sum(1).max()
+    assert bool(((got - want[:, None]).abs() <= bound[:, None]).all())
+    eight = (z.to(BF16).double() * sign.double()).sum(1)[c["index"][mine].long()]
+    assert bool(((eight - want[mine]).abs() > bound[mine]).any()), "a z of eight bits would be seen"
