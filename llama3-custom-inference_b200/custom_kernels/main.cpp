@@ -622,6 +622,9 @@ std::optional<Tensor> linear_rot_embed_kv_cache(Tensor x, Tensor w, Tensor freq,
   return q;
 }
 
+// Elements between the entries of an axis; nothing where there is but one, whose stride a view may leave at any number.
+int64_t step_of(const Tensor& t, int64_t axis) { return t.size(axis) == 1 ? 0 : t.stride(axis); }
+
 // What the calls on a paged cache share: caches [pages, page_size, n_kv_head, D] of equal layout, a table [B, entries] of page numbers, and
 // new tokens either as [B, T, ...] or, with `starts` (int32 [B + 1]), as packed rows.
 void check_paged(const Tensor& x, const Tensor& cache_k, const Tensor& cache_v, const Tensor& page_table, const Tensor& lengths, const char* lengths_name,
@@ -687,8 +690,8 @@ Tensor rot_embed_paged_kv_cache(Tensor qkv, Tensor freq, Tensor cache_k, Tensor 
   a.q_out = q.data_ptr(); a.cache_k = cache_k.data_ptr(); a.cache_v = cache_v.data_ptr();
   a.page_table = page_table.data_ptr<int32_t>(); a.positions = positions.data_ptr<int32_t>(); a.starts = starts ? starts->data_ptr<int32_t>() : nullptr;
   a.rows = starts ? qkv.size(0) : 0;
-  a.qkv_sb = starts ? 0 : qkv.stride(0); a.qkv_st = qkv.stride(-2); a.q_st = n_head * D;
-  a.freq_rows = freq.size(0); a.pages = cache_k.size(0); a.cache_sp = cache_k.stride(0); a.cache_st = cache_k.stride(1); a.table_st = page_table.stride(0);
+  a.qkv_sb = starts ? 0 : step_of(qkv, 0); a.qkv_st = step_of(qkv, -2); a.q_st = n_head * D;
+  a.freq_rows = freq.size(0); a.pages = cache_k.size(0); a.cache_sp = step_of(cache_k, 0); a.cache_st = step_of(cache_k, 1); a.table_st = page_table.stride(0);
   a.B = (int32_t)page_table.size(0); a.T = starts ? 0 : (int32_t)qkv.size(1); a.Hq = (int32_t)n_head; a.Hkv = (int32_t)n_kv_head; a.D = (int32_t)D;
   a.page_size = (int32_t)cache_k.size(1); a.max_pages = (int32_t)page_table.size(1);
   a.eps = (float)eps;
@@ -723,9 +726,9 @@ Tensor paged_attention(Tensor query, Tensor cache_k, Tensor cache_v, Tensor page
   a.q = query.data_ptr(); a.cache_k = cache_k.data_ptr(); a.cache_v = cache_v.data_ptr(); a.out = y.data_ptr();
   a.page_table = page_table.data_ptr<int32_t>(); a.seq_lens = seq_lens.data_ptr<int32_t>(); a.starts = starts ? starts->data_ptr<int32_t>() : nullptr;
   a.rows = starts ? query.size(0) : 0;
-  a.q_sb = starts ? 0 : query.stride(0); a.q_st = query.stride(-3); a.q_sh = query.stride(-2);
-  a.o_sb = starts ? 0 : y.stride(0); a.o_st = y.stride(-3); a.o_sh = y.stride(-2);
-  a.pages = cache_k.size(0); a.cache_sp = cache_k.stride(0); a.cache_st = cache_k.stride(1); a.table_st = page_table.stride(0);
+  a.q_sb = starts ? 0 : step_of(query, 0); a.q_st = step_of(query, -3); a.q_sh = step_of(query, -2);
+  a.o_sb = starts ? 0 : step_of(y, 0); a.o_st = step_of(y, -3); a.o_sh = step_of(y, -2);
+  a.pages = cache_k.size(0); a.cache_sp = step_of(cache_k, 0); a.cache_st = step_of(cache_k, 1); a.table_st = page_table.stride(0);
   a.B = (int32_t)page_table.size(0); a.T = starts ? 0 : (int32_t)query.size(1); a.Hq = (int32_t)query.size(-2); a.Hkv = (int32_t)cache_k.size(2); a.D = (int32_t)query.size(-1);
   a.page_size = (int32_t)cache_k.size(1); a.max_pages = (int32_t)page_table.size(1);
   a.scale = (float)scale;
