@@ -646,6 +646,7 @@ void check_paged(const Tensor& x, const Tensor& cache_k, const Tensor& cache_v, 
                 "starts must be a contiguous int32 CUDA tensor of shape [B + 1]");
   } else {
     TORCH_CHECK(x.size(0) == B, "the table must have a row for every sequence");
+    TORCH_CHECK(x.size(1) <= INT32_MAX, "tensor too large");
   }
   for (const Tensor* t : {&cache_k, &cache_v, &page_table, &lengths}) TORCH_CHECK(t->get_device() == x.get_device(), "tensors on different devices");
   TORCH_CHECK(!starts || starts->get_device() == x.get_device(), "tensors on different devices");

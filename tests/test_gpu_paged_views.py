@@ -1,4 +1,4 @@
-"""Views that the calls on paged caches take: an axis of one entry may carry any stride."""
+"""Views that the calls on paged caches take, an axis of one entry at any stride, and one that they refuse."""
 import pytest
 import torch
 
@@ -32,3 +32,12 @@ def test_axes_of_one_entry(ext, device, packed, T, Hq, Hkv):
     out = torch.zeros_like(y)
     ext.paged_attention(odd(want), *views, table, length, starts=starts, out=odd(out))
     assert torch.equal(out, y)
+
+
+def test_more_tokens_than_are_counted_in_32_bits(ext, device):
+    # (a broadcast token, which needs no memory; 2^32 + 1 is 1 in 32 bits)
+    k = torch.zeros(1, 16, 1, 8, dtype=BF16, device=device)
+    many = torch.zeros(1, 1, 24, dtype=BF16, device=device).expand(1, 2 ** 32 + 1, 24)
+    with pytest.raises(RuntimeError, match="too large"):
+        ext.rot_embed_paged_kv_cache(many, torch.zeros(16, 8, device=device), k, k.clone(), torch.zeros(1, 1, dtype=torch.int32, device=device),
+                                     torch.zeros(1, dtype=torch.int32, device=device), 1, 1)
