@@ -1,11 +1,14 @@
 // Low-rank adapters beside a shared projection (include/l3ci_b200.h, l3ci_adapter_linear): y = x w^T + z b^T, z = s x a^T by the adapters of the rows.
-// Two launches: z (fp32, in scratch), then the shared product with z b^T in its fp32 sums, one rounding at the end.  The second starts to read
-// w and x under the first.  Few rows (linear_rows.cu) are bound by the bytes of w: z b^T is multiply-adds of the output warps, a row of b a
-// thread, under the stream of w.  Many rows (linear_many.cu) are bound by the tensor cores: z b^T is two more products of a tile, z as the sum of two
+// Two launches: z (fp32, in scratch), then the shared product with z b^T in its fp32 sums, one rounding at the end.
+// Few rows (linear_rows.cu) are bound by the bytes of w, which the second launch reads, with x, while the first computes z: z b^T is multiply-adds
+// of the output warps, a row of b a thread, under the stream of w.  Many rows (linear_many.cu) are bound by the tensor cores, and read nothing before z
+// is complete: z b^T is two more products of a tile, z as the sum of two
 // bf16 (kept to 2^-16), for each adapter of the tile's rows in turn with the others' rows masked out of the instruction, not multiplied by zero.
-// Measured on a B200, calls back to back with changing weights: 8 rows of as many adapters of rank 16, 2048 -> 8192 10.1 us (34 MB of w: 3.3 TB/s; the kernel
-// alone 9.0); 64 rows, rank 32, 8192 -> 2048 16.4 (a
-// library's product alone 10.4 and 14.6); 6001 rows, rank 16, 2048 -> 8192 133 us for the product (1510 TFLOP/s) and 15 for z.
+// (A value of b that is infinite meets both halves of z there, and may give NaN where z b is infinite.)
+// Measured on a B200, calls one behind the other with changing weights: 8 rows of as many adapters of rank 16, 2048 -> 8192 10.1 us (34 MB of w: 3.3 TB/s; the
+// kernel alone 9.0); 64 rows of 8 adapters of rank 32, 8192 -> 2048 16.6, of 64 adapters 33 (a
+// library's product alone 10.4 and 14.6); 6001 rows of 6 adapters of rank 16, 2048 -> 8192 154 us in rows of 40 calls, 178 in long runs, at the power limit,
+// of which z takes 15 and the product 133 to 142 (1510 to 1420 TFLOP/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -217,7 +220,8 @@ namespace {
 // Whether the call goes to the product of few rows (64 at a time, weights on the wide side of the tensor cores, low-rank parts in multiply-adds) or to
 // that of many (tiles of 256 x 256 over pairs of SMs).  Estimates in us, fits to both sides on a B200, e.g. rank 16, 2 adapters, few and many: rows 128,
 // 2048 -> 8192 19 and 27, 512 62 and 27; 8192 -> 2048 rows 512 35 and 72; 4096 -> 4096 rows 256 21 and 42, 512 39 and 42; rank 64, 8
-// adapters: 2048 -> 8192 rows 128 41 and 55, 256 105 and 42.
+// adapters: 2048 -> 8192 rows 128 41 and 55, 256 105 and 42.  They know nothing of how many adapters a tile of rows has, which costs the product of
+// many rows a stage each: 256 rows, 2048 -> 8192, rank 16 of 1, 8, 64, 256 adapters 21, 36, 57, 163 us.
 bool few_rows(const l3ci_adapter_linear_args* a) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
   const long long groups = (a->rows + L3CI_LINEAR_MAX_ROWS - 1) / L3CI_LINEAR_MAX_ROWS;

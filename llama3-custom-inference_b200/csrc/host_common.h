@@ -66,8 +66,14 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // with the attribute that lets the grid be scheduled before the previous kernel of the stream has finished.  Kernels
 // launched this way call pdl_wait() (ptx_sm100.cuh) before they touch global memory: it returns once the previous
 // kernel has completed and its writes are visible, so the overlap is the launch itself, the CTAs' start and whatever
-// a kernel does before its first global access; a kernel launched the plain way passes through it at once.  One
-// kernel reads ahead of it: linear_rows_kernel its weights, if the caller vouches for them (l3ci_linear_args.early).
+// a kernel does before its first global access; a kernel launched the plain way passes through it at once.  These touch it ahead of that:
+//   * linear_rows_kernel its weights, if the caller vouches for them (l3ci_linear_args.early);
+//   * linear_rows_kernel with low-rank parts w and x, behind adapter_shrink_kernel or adapter_shrink_many_kernel;
+//   * paged_chunk_kernel all that it reads and writes, behind paged_rows_kernel of the same call, which writes other rows and another part of the scratch
+//     (it waits at its end, for the merge);
+//   * paged_merge_kernel lengths and starts, behind either.
+// The last three count on the kernel ahead in the same call: it calls pdl_wait() BEFORE pdl_launch_dependents(), so that all kernels before the
+// call have completed when they start.  pdl_begin() does it the other way round for small grids, and must not take the place of the two calls there.
 template <typename... Params, typename... Args>
 cudaError_t launch_kernel(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};

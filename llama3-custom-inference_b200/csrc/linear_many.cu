@@ -131,7 +131,7 @@ __device__ __forceinline__ void pair_mma_rows(uint32_t d, uint64_t a, uint64_t b
 // ADAPT: low-rank parts beside the product (l3ci_adapter_linear), as further columns: behind a tile's K columns come z of its rows as x and, for every
 // adapter among them, the adapter's b as w, in products that leave the rows of others alone; the parts land in the same accumulator and are
 // rounded once with it, and no row meets another's adapter (zeros in the place of other rows' z would, where a b is no number).  z is fp32: it goes in
-// as two bf16 that add up to 2^-17 of it, written by two warps of each CTA while the K columns run.
+// as two bf16 that add up to 2^-16 of it, written by two warps of each CTA while the K columns run.
 template <int ACT, bool ADAPT>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap bmap,

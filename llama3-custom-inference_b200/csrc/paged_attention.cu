@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const PagedPara
   const l3ci_paged_attention_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  pdl_wait();
+  pdl_wait();                // (in this order: the chunk kernel and the merge behind read what the kernels before have written, without a wait of their own)
   pdl_launch_dependents();
 
   count_columns<D>(p, pref);
@@ -521,7 +521,7 @@ __device__ __forceinline__ void merge_chunk(const ChunkParams& cp, int cta) {
   const PagedParams& p = cp.p;
   const l3ci_paged_attention_args& a = p.a;
   const int4 c0 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + cta / kShares<D> + 1)), c1 = __ldcg(reinterpret_cast<const int4*>(cp.cuts + cta / kShares<D> + 1) + 1);
-  const int b = c0.x, h = c0.y, m = c0.z, first = c0.w, parts = c1.y;
+  const int b = c0.x, h = c0.y, m = c0.z, first = c0.w, parts = c1.x;
   if (parts < 2) return;
   const PagedSeq s = paged_seq(p, b);
   const int t_unit = m * 2 * cp.tile_tokens;

@@ -49,8 +49,8 @@ __device__ __forceinline__ long long paged_row0(const PagedParams& p, int b, lon
 constexpr int kChunkRows = 128;
 // The unit that part g of the deal begins in the middle of, written by its CTA for the merge; parts 0: none, or its first cut is another part's.
 struct ChunkCut {
-  int b, h, m, first, last, parts;
-  int pad[2];
+  int b, h, m, first, parts;
+  int pad[3];
 };
 struct ChunkParams {
   PagedParams p;

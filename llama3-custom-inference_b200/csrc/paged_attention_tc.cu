@@ -12,8 +12,9 @@
 //   * what lies behind a sequence's end in its last page, and values that some rows of a tile must not see, may be no numbers, and a
 //     weight of 0 does not stop them: two guard warps look through V tiles at the diagonal and the end, under the first product and the softmax
 //     of the same tile, take such values out, and the output group adds them to the rows that see them.
-// Measured on a B200: 2 x 512 tokens of 16500 keys, 32 query on 8 KV heads of 128, any page size 243 us, 1120 TFLOP/s, heads of 64 202, 675; a prompt of
-// 4096 tokens, heads of 128 155 us, 890, of 64 121, 570 (a head of 64 has half the products to the same exponentials).  A tile of keys takes
+// Measured on a B200, rows of 40 calls, merge included: 2 x 512 tokens of 16500 keys, 32 query on 8 KV heads of 128, 241 us, 1130 TFLOP/s (284, 960, in long
+// runs, at the power limit), heads of 64 192, 711; a prompt of
+// 4096 tokens, heads of 128 157 us, 876, of 64 115, 600 (a head of 64 has half the products to the same exponentials).  A tile of keys takes
 // 3650 cycles (heads of 128), of which a warp's softmax is 2030 (its exponentials alone 1450 for the 1024 that they cannot do without) and
 // the wait for the products between 1240; the tensor cores need 2050 and the exponentials of both groups as much.  For heads of 64 the weights
 // in a place of their own, so that the next scores come under the exponentials: both groups then take theirs at once, 234 us instead of 227 (of 202
@@ -151,7 +152,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_launch_dependents();
+  pdl_launch_dependents();   // (behind pdl_wait, here or in paged_rows_kernel: the merge reads lengths and starts before its own)
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_s[2] = {tmem, tmem + 128u};
   const uint32_t t_o[2] = {tmem + 256u, tmem + 256u + (uint32_t)D};
@@ -228,8 +229,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           cut.b = u.b;
           cut.h = u.h;
           cut.m = u.m;
-          cut.last = fd_cta_of(u.first + kUnitCost + kTileCost * (u.tiles - 1), total, parts);
-          cut.parts = cut.last - cut.first + 1;
+          cut.parts = fd_cta_of(u.first + kUnitCost + kTileCost * (u.tiles - 1), total, parts) - cut.first + 1;
         }
       }
       cp.cuts[part] = cut;
@@ -309,7 +309,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
     // ---- MMA issue: all lanes run the code, one issues the instructions; what all lanes agree on comes out of a shuffle, so that the compiler knows it too
     // (elect_one).  With `lane == 0` and plain registers this warp bounded the kernel: 2 x 512 tokens of 16500 keys of 32 heads of 128 took 283 us
-    // instead of 243 (960 and 1120 TFLOP/s), a prompt of 4096 tokens of heads of 64 142 instead of 130 ----
+    // instead of 243 (short runs; 960 and 1120 TFLOP/s), a prompt of 4096 tokens of heads of 64 142 instead of 130 ----
     constexpr uint32_t idesc_qk = instr_desc(kRows, kKeys, false);
     constexpr uint32_t idesc_pv = instr_desc(kRows, D, true);
     const uint32_t elected = elect_one();
