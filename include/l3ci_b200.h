@@ -404,7 +404,7 @@ L3CI_API int l3ci_flash_decode_exchange(const l3ci_flash_decode_args* args, void
  * pages cache_sp and tokens cache_st elements apart, the same in both); token p of sequence b lies in row p % page_size of
  * page page_table[b * table_st + p / page_size].  A batch of new tokens is either B sequences of T tokens each, or, with
  * `starts` (int32 [B + 1], ascending), packed rows: sequence b has rows [starts[b], starts[b + 1]), and rows from
- * starts[B] on belong to nobody and are left as they were.  Positions, lengths, starts and tables are read on the device alone,
+ * starts[B] on belong to nobody and are left as they were.  (Where `starts` does not ascend, which rows are written is not said; none out of place.)  Positions, lengths, starts and tables are read on the device alone,
  * so that a step can be captured in a CUDA graph; an entry of the table that is not in [0, pages) is a page that is not there.
  * No counterpart in the reference, whose caches are [maxB, maxLen, Hkv, D] (model.py:105-108).
  * ------------------------------------------------------------------------------------------ */

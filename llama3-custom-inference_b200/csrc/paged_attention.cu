@@ -609,7 +609,7 @@ int check(const l3ci_paged_attention_args* a) {
   // (columns of a sequence, 16 keys of a head each, are counted in 32 bits)
   if (rows > 0x7fffffffLL || a->pages > 0x7fffffffLL || (long long)a->max_pages * a->page_size > (1LL << 30) / (a->Hkv < 16 ? 16 : a->Hkv) * 16)
     return fail(L3CI_ERR_INVALID, "paged_attention: %lld rows, %lld keys a sequence", rows, (long long)a->max_pages * a->page_size);
-  if ((a->starts ? a->rows : a->T) * (a->Hq / a->Hkv) > kFewRows && paged_chunk_columns(a) > 0x7fffffffLL)
+  if ((a->starts ? a->rows : a->T) * (a->Hq / a->Hkv) > kFewRows && paged_chunk_columns(a) >= 0x7fffffffLL)
     return fail(L3CI_ERR_INVALID, "paged_attention: %lld rows over up to %lld keys are too many for one call", rows, (long long)a->max_pages * a->page_size);
   return L3CI_OK;
 }

@@ -121,6 +121,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
   if (!cp.follows) pdl_wait();
   // ---- columns of the deal before every sequence ----
+  // (The host has seen that the rows of the call, each counted once, stay below 2^31.  `starts` that do not ascend may name rows again and again: a sum that
+  // gets there stays there, and nothing is done.)
+  constexpr int kMost = 0x7fffffff;
+  auto add = [](int x, int y) { return (int)min((unsigned)x + (unsigned)y, (unsigned)kMost); };
   constexpr int kUnitCost = unit_cost(D);
   const int block = 2 * cp.tile_tokens;
   auto columns_of_head = [&](const PagedSeq& s) {
@@ -134,20 +138,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     for (int b = b0; b < b1; ++b) {
       const int c = a.Hkv * columns_of_head(paged_seq(p, b));
       pref[b + 1] = c;
-      mine += c;
+      mine = add(mine, c);
     }
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int other = __shfl_up_sync(kFullMask, upto, d);
-      if (lane >= d) upto += other;
+      if (lane >= d) upto = add(upto, other);
     }
     if (lane == 31) sums[warp] = upto;
     if (threadIdx.x == 0) pref[0] = 0;
     __syncthreads();
     int before = upto - mine;
-    for (int w = 0; w < warp; ++w) before += sums[w];
-    for (int b = b0; b < b1; ++b) pref[b + 1] = before += pref[b + 1];
+    for (int w = 0; w < warp; ++w) before = add(before, sums[w]);
+    for (int b = b0; b < b1; ++b) pref[b + 1] = before = add(before, pref[b + 1]);
   }
   tc_fence_before();
   __syncthreads();
@@ -156,7 +160,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_s[2] = {tmem, tmem + 128u};
   const uint32_t t_o[2] = {tmem + 256u, tmem + 256u + (uint32_t)D};
-  const int total = pref[a.B], parts = max(min(total / kTileCost, p.max_parts), 1), part = blockIdx.x;   // (no run between two tiles' first columns)
+  const int total = pref[a.B] == kMost ? 0 : pref[a.B], parts = max(min(total / kTileCost, p.max_parts), 1), part = blockIdx.x;   // (no run between two tiles' first columns)
   const int begin = total > 0 && part < parts ? fd_range_begin(part, total, parts) : 0, end = total > 0 && part < parts ? fd_range_begin(part + 1, total, parts) : 0;
 
   // the next segment; false: the wait for it ran out
